@@ -106,6 +106,34 @@ pub struct rmlk_row_stream {
     pub partial_stride: i64,
 }
 
+/// A paged int8 cache of keys and values (see `rmlk_hip_paged_append`).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rmlk_paged_cache {
+    pub pages: i64,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+}
+
+/// The ragged sequences of one call over a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rmlk_paged_batch {
+    pub seqs: i64,
+    pub rows: i64,
+    pub max_new: i64,
+    pub max_length: i64,
+    pub table_stride: i64,
+    pub first: *const i32,
+    pub length: *const i32,
+    pub page_table: *const i32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy)]
 pub struct rmlk_device_info {
@@ -124,6 +152,7 @@ SCALARS = {
     "int32_t": "i32", "int64_t": "i64", "size_t": "usize", "float": "f32", "double": "f64",
     "rmlk_stream_t": "rmlk_stream_t", "void": "c_void", "char": "c_char", "uint8_t": "u8", "uint64_t": "u64",
     "rmlk_dims": "rmlk_dims", "rmlk_row_stream": "rmlk_row_stream", "rmlk_device_info": "rmlk_device_info",
+    "rmlk_paged_cache": "rmlk_paged_cache", "rmlk_paged_batch": "rmlk_paged_batch",
 }
 RESERVED = {"in": "input", "type": "kind", "ref": "reference", "fn": "func", "mod": "modulus"}
 

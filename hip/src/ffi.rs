@@ -88,6 +88,34 @@ pub struct rmlk_row_stream {
     pub partial_stride: i64,
 }
 
+/// A paged int8 cache of keys and values (see `rmlk_hip_paged_append`).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rmlk_paged_cache {
+    pub pages: i64,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+}
+
+/// The ragged sequences of one call over a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rmlk_paged_batch {
+    pub seqs: i64,
+    pub rows: i64,
+    pub max_new: i64,
+    pub max_length: i64,
+    pub table_stride: i64,
+    pub first: *const i32,
+    pub length: *const i32,
+    pub page_table: *const i32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy)]
 pub struct rmlk_device_info {
@@ -807,6 +835,90 @@ extern "C" {
         n_streams: i32,
         streams: *const rmlk_row_stream,
         first_col: *const i64,
+        err_flag: *mut i32,
+    ) -> i32;
+    pub fn rmlk_hip_quantize_rows(
+        stream: rmlk_stream_t,
+        dtype: i32,
+        rows: i64,
+        cols: i64,
+        x: *const c_void,
+        ldx: i64,
+        q: *mut c_void,
+        ldq: i64,
+        scale: *mut f32,
+    ) -> i32;
+    pub fn rmlk_hip_rmsnorm_quantize_rows(
+        stream: rmlk_stream_t,
+        dtype: i32,
+        rows: i64,
+        cols: i64,
+        x: *const c_void,
+        b: *const c_void,
+        gamma: *const f32,
+        eps: f32,
+        sum_out: *mut c_void,
+        q: *mut c_void,
+        ldq: i64,
+        scale: *mut f32,
+    ) -> i32;
+    pub fn rmlk_hip_matmul_int8_workspace_size(m: i64, n: i64, k: i64) -> usize;
+    pub fn rmlk_hip_matmul_int8(
+        stream: rmlk_stream_t,
+        dtype: i32,
+        m: i64,
+        n: i64,
+        k: i64,
+        a: *const c_void,
+        lda: i64,
+        a_scale: *const f32,
+        wt: *const c_void,
+        ldw: i64,
+        w_scale: *const f32,
+        residual: *const c_void,
+        ldr: i64,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        c: *mut c_void,
+        ldc: i64,
+    ) -> i32;
+    pub fn rmlk_hip_paged_append(
+        stream: rmlk_stream_t,
+        dtype: i32,
+        cache: *const rmlk_paged_cache,
+        batch: *const rmlk_paged_batch,
+        k: *const c_void,
+        k_stride: i64,
+        v: *const c_void,
+        v_stride: i64,
+        cos: *const f32,
+        sin: *const f32,
+        positions: i64,
+        heads: i64,
+        q: *const c_void,
+        q_stride: i64,
+        q_out: *mut c_void,
+        err_flag: *mut i32,
+    ) -> i32;
+    pub fn rmlk_hip_paged_attention_workspace_size(
+        dtype: i32,
+        cache: *const rmlk_paged_cache,
+        batch: *const rmlk_paged_batch,
+        heads: i64,
+    ) -> usize;
+    pub fn rmlk_hip_paged_attention(
+        stream: rmlk_stream_t,
+        dtype: i32,
+        cache: *const rmlk_paged_cache,
+        batch: *const rmlk_paged_batch,
+        heads: i64,
+        q: *const c_void,
+        q_stride: i64,
+        scale_is_mul: i32,
+        scale: f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        out: *mut c_void,
         err_flag: *mut i32,
     ) -> i32;
     pub fn rmlk_hip_batch_begin(stream: rmlk_stream_t) -> i32;

@@ -44,7 +44,7 @@ typedef enum rmlk_status {
     RMLK_ERR_NULL_POINTER = -3,    /* null pointer with a non-zero length */
     RMLK_ERR_SIZE_MISMATCH = -4,   /* shapes / lengths disagree */
     RMLK_ERR_INVALID_ARGUMENT = -5,/* bad axis, perm, step 0, negative dim ... */
-    RMLK_ERR_WORKSPACE = -6,       /* workspace smaller than rmlk_hip_matmul_workspace_size says */
+    RMLK_ERR_WORKSPACE = -6,       /* workspace smaller than the call's *_workspace_size says */
     RMLK_ERR_TOO_LARGE = -7,       /* more elements than the kernels index (>= 2^62) */
     RMLK_ERR_SCRATCH_LIMIT = -8    /* rmlk_hip_matmul_noalloc: the problem needs more scratch than the
                                       library's fixed array holds */
@@ -65,7 +65,8 @@ typedef enum rmlk_dtype {
     RMLK_DOUBLE = 11,
     RMLK_UINT32 = 12,
     RMLK_UINT64 = 13,
-    RMLK_BFLOAT16 = 16 /* only as the storage type of constant weights (w_dtype below) */
+    RMLK_BFLOAT16 = 16 /* only as the storage type of constant weights (w_dtype below) and as the
+                          activation type of the 8-bit operators */
 } rmlk_dtype;
 
 /* Shape or stride vector passed by value from the host; replaces the device `info` buffers the
@@ -645,6 +646,112 @@ int32_t rmlk_hip_gemv_kmajor_head_rows(rmlk_stream_t stream, int32_t dtype, int6
                                        int32_t w_dtype, const void *wt, int64_t ldw, int32_t n_streams,
                                        const rmlk_row_stream *streams, const int64_t *first_col,
                                        int32_t *err_flag);
+
+/* ---- 8-bit serving: int8 rows, int8 products, a paged int8 cache ------------------------------------
+ * Activations (`dtype`: x, q, k, v, residual and the outputs of that kind) are FLOAT, FLOAT16 or
+ * BFLOAT16; sums, softmax statistics and norms are formed in 32 bits or more and rounded once. No
+ * counterpart in the reference, whose kernels hold fp32 only.
+ *
+ * rmlk_hip_quantize_rows: one scale per row (a token's activations, or an output channel's weights),
+ *   scale[r] = float(max|x[r, :]| / 127),  q[r, j] = x[r, j] / scale[r] rounded to nearest even,
+ * decided as in exact arithmetic; |q| <= 127. A row whose largest magnitude lies below 2^-100 gets
+ * scale 0 and q 0; a row that holds a NaN or an infinity gets scale NaN and q 0, so that what is
+ * computed from it is NaN. x has rows of `cols` values ldx apart, q rows ldq bytes apart with ldq a
+ * multiple of 16, ldq >= cols; bytes cols .. cols rounded up to 16 of a row are set to zero.
+ * rmlk_hip_rmsnorm_quantize_rows: the same of y = x / sqrt(mean(x^2) + eps) * gamma (evaluated in
+ * double), with b given of x + b, which is rounded to `dtype`, stored to sum_out and normalised from
+ * there. x, b, sum_out dense [rows, cols] (sum_out may be x or b), gamma float [cols]; b and sum_out
+ * are both given or both NULL.
+ * Chain: [Add] -> Pow, ReduceMean, Add, Sqrt, Div, Mul -> the quantisation. */
+int32_t rmlk_hip_quantize_rows(rmlk_stream_t stream, int32_t dtype, int64_t rows, int64_t cols,
+                               const void *x, int64_t ldx, void *q, int64_t ldq, float *scale);
+int32_t rmlk_hip_rmsnorm_quantize_rows(rmlk_stream_t stream, int32_t dtype, int64_t rows, int64_t cols,
+                                       const void *x, const void *b, const float *gamma, float eps,
+                                       void *sum_out, void *q, int64_t ldq, float *scale);
+
+/* c[i, j] = (sum_k a[i, k] * wt[j, k]) * a_scale[i] * w_scale[j] (+ residual[i, j]), rounded to `dtype`:
+ * a int8 [m, k] (rows lda bytes apart, one scale per token), wt int8 [n, k] (K-contiguous, rows ldw
+ * apart, one scale per channel), as rmlk_hip_quantize_rows leaves both. The integer sums are exact.
+ * residual (NULL: none) has rows ldr elements apart (0: one row for all, i.e. a bias) and may be c.
+ * lda and ldw are multiples of 16 and at least k rounded up to 16, a and wt 16-byte aligned
+ * (RMLK_ERR_UNSUPPORTED otherwise); what the bytes k .. of a row hold does not matter. k < 131072
+ * (larger sums could leave 32 bits: RMLK_ERR_TOO_LARGE). The workspace holds
+ * rmlk_hip_matmul_int8_workspace_size bytes (0 for most sizes), 16-byte aligned; its contents on
+ * entry do not matter and it belongs to the call until its kernels have run. */
+size_t rmlk_hip_matmul_int8_workspace_size(int64_t m, int64_t n, int64_t k);
+int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int64_t n, int64_t k,
+                             const void *a, int64_t lda, const float *a_scale, const void *wt,
+                             int64_t ldw, const float *w_scale, const void *residual, int64_t ldr,
+                             void *workspace, size_t workspace_bytes, void *c, int64_t ldc);
+
+/* A cache of keys and values in pages, held in 8 bits. A block (one page of one KV head) stores int8
+ * values and one scale for K and one for V; a scale is a power of two, so that a value can be
+ * re-rounded to a larger scale any number of times and stays within one (final) step of what was
+ * appended: s/2 + s/4 + .. < s. page_size is 16, 32, 64 or 128, head_dim 64 or 128. V lies
+ * transposed: the attention reads sixteen tokens of one head dim at a time. All arrays 16-byte
+ * aligned. The caller owns them; a page needs no initialisation before its first append. */
+typedef struct rmlk_paged_cache {
+    int64_t pages;          /* pages the arrays hold */
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    void *k;                /* int8  [pages, kv_heads, page_size, head_dim] */
+    void *v;                /* int8  [pages, kv_heads, head_dim, page_size] */
+    float *k_scale;         /* float [pages, kv_heads] */
+    float *v_scale;
+} rmlk_paged_cache;
+/* The sequences of one call, ragged: rows first[s] .. first[s + 1] of q, k, v and out are the newest
+ * tokens of sequence s, which then holds length[s] tokens; token t lies in page
+ * page_table[s * table_stride + t / page_size]. The three arrays are DEVICE memory; max_new and max_length
+ * are bounds of the caller's on a sequence's rows and length (they shape the launch). What the arrays
+ * hold is checked on the device and reported by 1 in *err_flag (device int32, may be NULL): `first` that
+ * does not ascend within 0 .. rows, nothing is done then; a sequence whose rows or length leave the
+ * bounds or the page table, it is skipped; an index of a page outside the cache, that page's tokens
+ * are. Rows behind first[seqs] (a padded batch) and slots behind a sequence's tokens stay as they
+ * are. */
+typedef struct rmlk_paged_batch {
+    int64_t seqs;
+    int64_t rows;           /* rows q, k, v and out hold */
+    int64_t max_new;
+    int64_t max_length;
+    int64_t table_stride;   /* pages per sequence in the table */
+    const int32_t *first;   /* [seqs + 1] */
+    const int32_t *length;  /* [seqs], the new tokens included */
+    const int32_t *page_table;
+} rmlk_paged_batch;
+
+/* Appends the new tokens: k and v [rows, kv_heads, head_dim] (rows k_stride / v_stride elements apart),
+ * k rotated like rmlk_hip_rotary with row t of the tables cos and sin, float [positions, head_dim], t the
+ * token's position in its sequence (both NULL: k as it is; a token at a position >= positions is
+ * skipped and reported, as is a sequence of fewer tokens than rows). A block's scale becomes the smallest power of two s with |x| <= 127 s for everything
+ * appended to it, at least 2^-126; an append that starts at slot 0 of a page starts its blocks anew,
+ * whatever they held. Rounding to nearest even, decided as in exact arithmetic. A NaN or an infinity
+ * among a block's new values makes its scale NaN until the block is started anew, and the attention of
+ * every query that sees a token of the block NaN. q (NULL: none), [rows, heads, head_dim], is rotated
+ * alike into the dense q_out (may be q). A page that receives tokens belongs to one sequence of the
+ * call. 16-byte aligned rows, heads a multiple of kv_heads; RMLK_ERR_UNSUPPORTED otherwise. */
+int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_paged_cache *cache,
+                              const rmlk_paged_batch *batch, const void *k, int64_t k_stride,
+                              const void *v, int64_t v_stride, const float *cos, const float *sin,
+                              int64_t positions, int64_t heads, const void *q, int64_t q_stride,
+                              void *q_out, int32_t *err_flag);
+
+/* out[i, h, :] = Softmax_t(q[i, h, :] . k[t, h / rep, :] * scale) . v[t, h / rep, :] over the cached tokens
+ * t <= the position of row i in its sequence, rep = heads / kv_heads (scale_is_mul == 0: the scores are
+ * DIVIDED by scale, as in rmlk_hip_attention). One call serves prompts, chunks of prompts behind what is
+ * cached and single tokens alike. A query that sees nothing (its position is negative: more rows than
+ * tokens) gives zeros. q has rows q_stride elements apart, out is dense [rows, heads, head_dim]; q is read
+ * as one (16-bit types) or two half values (float, 22 significant bits relative to the row's largest)
+ * and the cached integers exactly; scales that are no powers of two are rounded to 11 bits in V. The
+ * workspace holds rmlk_hip_paged_attention_workspace_size bytes, 16-byte aligned (0 where the keys
+ * are not split over blocks); its contents on entry do not matter, and it belongs to the call until its
+ * kernels have run. */
+size_t rmlk_hip_paged_attention_workspace_size(int32_t dtype, const rmlk_paged_cache *cache,
+                                               const rmlk_paged_batch *batch, int64_t heads);
+int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk_paged_cache *cache,
+                                 const rmlk_paged_batch *batch, int64_t heads, const void *q,
+                                 int64_t q_stride, int32_t scale_is_mul, float scale, void *workspace,
+                                 size_t workspace_bytes, void *out, int32_t *err_flag);
 
 /* ---- launches over tiny tensors collected into one ------------------------------------------------
  * Between rmlk_hip_batch_begin and rmlk_hip_batch_end on a stream, calls of rmlk_hip_binary (not

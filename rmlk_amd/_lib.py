@@ -47,6 +47,18 @@ class RowStream(ctypes.Structure):
                 ("partials", c_int32), ("partial_stride", c_int64)]
 
 
+class PagedCacheStruct(ctypes.Structure):
+    """struct rmlk_paged_cache"""
+    _fields_ = [("pages", c_int64), ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    """struct rmlk_paged_batch"""
+    _fields_ = [("seqs", c_int64), ("rows", c_int64), ("max_new", c_int64), ("max_length", c_int64),
+                ("table_stride", c_int64), ("first", c_void_p), ("length", c_void_p), ("page_table", c_void_p)]
+
+
 class DeviceInfo(ctypes.Structure):
     """struct rmlk_device_info"""
     _fields_ = [("name", ctypes.c_char * 128), ("arch", ctypes.c_char * 64),
@@ -186,6 +198,22 @@ SIGNATURES = {
     "rmlk_hip_gemv_kmajor_head_rows": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_void_p, ctypes.c_float,
                                                  c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p,
                                                  c_void_p, c_void_p]),
+    "rmlk_hip_quantize_rows": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                         c_void_p]),
+    "rmlk_hip_rmsnorm_quantize_rows": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                                 ctypes.c_float, c_void_p, c_void_p, c_int64, c_void_p]),
+    "rmlk_hip_matmul_int8_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "rmlk_hip_matmul_int8": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                       c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_size_t,
+                                       c_void_p, c_int64]),
+    "rmlk_hip_paged_append": (c_int32, [c_void_p, c_int32, POINTER(PagedCacheStruct), POINTER(PagedBatchStruct),
+                                        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_void_p]),
+    "rmlk_hip_paged_attention_workspace_size": (c_size_t, [c_int32, POINTER(PagedCacheStruct),
+                                                           POINTER(PagedBatchStruct), c_int64]),
+    "rmlk_hip_paged_attention": (c_int32, [c_void_p, c_int32, POINTER(PagedCacheStruct), POINTER(PagedBatchStruct),
+                                           c_int64, c_void_p, c_int64, c_int32, ctypes.c_float, c_void_p, c_size_t,
+                                           c_void_p, c_void_p]),
     "rmlk_hip_batch_begin": (c_int32, [c_void_p]),
     "rmlk_hip_batch_flush": (c_int32, [c_void_p]),
     "rmlk_hip_batch_end": (c_int32, [c_void_p]),

@@ -1,0 +1,165 @@
+// What the kernels of the 8-bit serving path share: activation types and the paged int8 cache.
+#pragma once
+
+#include "common.hpp"
+
+namespace rmlk {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Activation types: float, _Float16, __bf16. to_float is exact, from_float rounds to nearest even.
+typedef _Float16 half_t;
+typedef __bf16 bf16_t;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x) {
+    return static_cast<float>(x);
+}
+
+// N values of type T (N * sizeof(T) a multiple of 16 bytes) from a 16-byte aligned address, widened.
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const T *p, float (&out)[N]) {
+    static_assert(N * sizeof(T) % 16 == 0, "whole 16-byte units");
+    T v[N];
+#pragma unroll
+    for (size_t i = 0; i < N * sizeof(T) / 16; ++i)
+        reinterpret_cast<u32x4 *>(v)[i] = reinterpret_cast<const u32x4 *>(p)[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_float(v[i]);
+}
+
+inline bool is_activation(int32_t dtype) {
+    return dtype == RMLK_FLOAT || dtype == RMLK_FLOAT16 || dtype == RMLK_BFLOAT16;
+}
+
+// f(T{}) with the element type of an activation dtype.
+template <typename F>
+inline int32_t with_activation(int32_t dtype, F &&f) {
+    switch (dtype) {
+        case RMLK_FLOAT: return f(float{});
+        case RMLK_FLOAT16: return f(half_t{});
+        case RMLK_BFLOAT16: return f(bf16_t{});
+        default: return RMLK_ERR_UNSUPPORTED;
+    }
+}
+
+inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+struct PagedArgs {
+    int8_t *k;
+    int8_t *v;
+    float *k_scale;
+    float *v_scale;
+    const int32_t *first;
+    const int32_t *length;
+    const int32_t *table;
+    int64_t table_stride;
+    int64_t rows;
+    int64_t pages;
+    int64_t max_new, max_length;
+    int32_t seqs;
+    int32_t kv_heads;
+    int32_t page_shift;      // log2 of the page size
+    int32_t *err;
+};
+
+// Argument checks of the two structs, and the kernel arguments they give.
+inline int32_t paged_args(const rmlk_paged_cache *cache, const rmlk_paged_batch *batch, int32_t *err_flag,
+                          PagedArgs *g) {
+    if (!cache || !batch) return RMLK_ERR_NULL_POINTER;
+    if (cache->pages < 0 || cache->kv_heads < 1 || batch->seqs < 0 || batch->rows < 0 || batch->max_new < 0 ||
+        batch->max_length < 0 || batch->table_stride < 0)
+        return RMLK_ERR_INVALID_ARGUMENT;
+    const int32_t ps = cache->page_size;
+    if ((ps != 16 && ps != 32 && ps != 64 && ps != 128) || (cache->head_dim != 64 && cache->head_dim != 128))
+        return RMLK_ERR_UNSUPPORTED;
+    // what the kernels count with 32 bits
+    if (cache->pages > 0x7fffffff || batch->seqs > 0xffff || cache->kv_heads > 0xffff ||
+        batch->rows > 0x3fffffff || batch->max_length > 0x3fffffff || batch->max_new > 0x3fffffff)
+        return RMLK_ERR_TOO_LARGE;
+    g->k = static_cast<int8_t *>(cache->k);
+    g->v = static_cast<int8_t *>(cache->v);
+    g->k_scale = cache->k_scale;
+    g->v_scale = cache->v_scale;
+    g->first = batch->first;
+    g->length = batch->length;
+    g->table = batch->page_table;
+    g->table_stride = batch->table_stride;
+    g->rows = batch->rows;
+    g->pages = cache->pages;
+    g->max_new = batch->max_new < batch->rows ? batch->max_new : batch->rows;
+    const int64_t room = batch->table_stride > (0x3fffffff / ps) ? 0x3fffffff : batch->table_stride * ps;
+    g->max_length = batch->max_length < room ? batch->max_length : room;
+    g->seqs = static_cast<int32_t>(batch->seqs);
+    g->kv_heads = cache->kv_heads;
+    g->page_shift = ps == 16 ? 4 : ps == 32 ? 5 : ps == 64 ? 6 : 7;
+    g->err = err_flag;
+    return RMLK_OK;
+}
+
+// The pointers of a call that has something to do.
+inline int32_t paged_pointers(const rmlk_paged_cache *cache, const rmlk_paged_batch *batch) {
+    if (!batch->first || !batch->length) return RMLK_ERR_NULL_POINTER;
+    if (batch->table_stride > 0 && !batch->page_table) return RMLK_ERR_NULL_POINTER;
+    if (cache->pages > 0 && (!cache->k || !cache->v || !cache->k_scale || !cache->v_scale))
+        return RMLK_ERR_NULL_POINTER;
+    if (!aligned16(cache->k) || !aligned16(cache->v)) return RMLK_ERR_UNSUPPORTED;
+    return RMLK_OK;
+}
+
+// Rows, new tokens and length of sequence s; false for one whose numbers contradict the call's bounds.
+struct Sequence {
+    int32_t row;       // its first row
+    int32_t fresh;     // its rows
+    int32_t length;    // tokens it holds, these included
+};
+__device__ __forceinline__ bool sequence_at(const PagedArgs &g, int s, Sequence &q) {
+    const int32_t lo = g.first[s], hi = g.first[s + 1];
+    q.row = lo;
+    q.fresh = hi - lo;
+    q.length = g.length[s];
+    return lo >= 0 && hi >= lo && hi <= g.rows && hi - lo <= g.max_new && q.length >= 0 && q.length <= g.max_length;
+}
+
+// first[0 .. seqs] ascends within 0 .. rows (checked by every wavefront for itself: the array is a few
+// cache lines).
+__device__ __forceinline__ bool starts_ascend(const PagedArgs &g) {
+    bool good = true;
+    for (int i = static_cast<int>(threadIdx.x % kWave); i < g.seqs; i += kWave) {
+        const int32_t lo = g.first[i], hi = g.first[i + 1];
+        good = good && lo >= 0 && lo <= hi && hi <= g.rows;
+    }
+    return __all(good);
+}
+
+// The work of a ragged call in pieces of `unit` (a power of two or not) rows: sequence s has the numbers
+// from first[s] / unit + extra * s on, floor(rows / unit) + extra of them at least, so that a grid of
+// rows / unit + extra * seqs blocks covers every sequence without a rectangle over the longest one.
+// A wavefront counts the sequences that begin at or before `piece`; -1 with no sequence.
+__device__ __forceinline__ int sequence_of(const PagedArgs &g, int piece, int unit, int extra) {
+    int s = -1;
+    for (int base = 0; base < g.seqs; base += kWave) {
+        const int i = base + static_cast<int>(threadIdx.x % kWave);
+        s += __popcll(__ballot(i < g.seqs && g.first[i] / unit + extra * i <= piece));
+    }
+    return s;
+}
+
+// The last sequence that starts at or before a row (of those that share a start: the last, which is
+// the one that has rows).
+__device__ __forceinline__ int sequence_of_row(const PagedArgs &g, int64_t row) {
+    int lo = 0, hi = g.seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (g.first[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void raise_error(const PagedArgs &g) {
+    if (g.err) *g.err = 1;
+}
+
+}  // namespace rmlk

@@ -17,7 +17,7 @@ from ._lib import Dims, RmlkError, check, lib
 # ONNX TensorProto.DataType numbers (include/rmlk_hip.h rmlk_dtype)
 FLOAT, UINT8, INT8, UINT16, INT16, INT32, INT64, BOOL, FLOAT16, DOUBLE, UINT32, UINT64 = (
     1, 2, 3, 4, 5, 6, 7, 9, 10, 11, 12, 13)
-BFLOAT16 = 16   # only as the storage type of constant weights
+BFLOAT16 = 16   # storage type of constant weights, activation type of the 8-bit operators
 
 TORCH_TO_DTYPE = {
     torch.float32: FLOAT, torch.uint8: UINT8, torch.int8: INT8, torch.int16: INT16,
@@ -47,7 +47,8 @@ def dtype_of(t: torch.Tensor) -> int:
 
 
 def storage_of(w: torch.Tensor) -> int:
-    """Storage type of a weight matrix handed to the products over constant weights."""
+    """Storage type of a weight matrix handed to the products over constant weights (and the activation
+    type of the 8-bit operators)."""
     return BFLOAT16 if w.dtype == torch.bfloat16 else TORCH_TO_DTYPE[w.dtype]
 
 
@@ -512,6 +513,161 @@ def gemv_kmajor_head_rows(x, wt, k: int, streams, first_cols, gamma=None, eps: f
                                                arr, cols,
                                                _ptr(err_flag) if err_flag is not None else None),
           "rmlk_hip_gemv_kmajor_head_rows")
+
+
+# ---- 8-bit serving: int8 rows and products, a paged int8 cache ----------------------------------------
+
+def _rows(t, width: int) -> int:
+    """Elements from one row to the next of a tensor [rows, ...] whose rows hold `width` dense elements."""
+    dense = 1
+    for d in range(t.dim() - 1, 0, -1):
+        assert t.shape[d] == 1 or t.stride(d) == dense, "the elements of a row must be dense"
+        dense *= t.shape[d]
+    assert dense == width, f"rows hold {dense} elements, {width} expected"
+    _here(t)
+    return max(t.stride(0), width) if t.shape[0] > 1 else width
+
+
+def _here(*tensors) -> None:
+    """The launch goes to the current stream of the current device: its operands have to lie there."""
+    for t in tensors:
+        if t is not None:
+            assert t.is_cuda and t.device.index == torch.cuda.current_device(), "tensors must lie on the current device"
+
+
+def quantize_rows(x, q, scale) -> None:
+    """q int8 [rows, ld] (ld: cols rounded up to 16, or more) and scale float [rows] of x [rows, cols] (float,
+    float16 or bfloat16; rows may lie apart): scale = max|row| / 127, q = row / scale to nearest even."""
+    rows, cols = x.shape
+    _here(q, scale)
+    assert q.dtype == torch.int8 and q.shape[0] == rows and q.stride(1) == 1 and q.shape[1] >= (cols + 15) // 16 * 16
+    assert scale.dtype == torch.float32 and scale.numel() == rows
+    check(lib().rmlk_hip_quantize_rows(_stream(), storage_of(x), rows, cols, x.data_ptr(), _rows(x, cols),
+                                       q.data_ptr(), _rows(q, q.shape[1]), _ptr(scale)), "rmlk_hip_quantize_rows")
+
+
+def rmsnorm_quantize_rows(x, gamma, eps: float, q, scale, add=None, sum_out=None) -> None:
+    """quantize_rows of x / sqrt(mean(x^2) + eps) * gamma; with `add` of x + add, which also goes to sum_out."""
+    rows, cols = x.shape
+    _here(x, gamma, q, scale, add, sum_out)
+    assert q.dtype == torch.int8 and q.shape[0] == rows and q.stride(1) == 1 and q.shape[1] >= (cols + 15) // 16 * 16
+    assert scale.dtype == torch.float32 and scale.numel() == rows
+    assert gamma.dtype == torch.float32 and gamma.numel() == cols
+    for t in (add, sum_out):
+        assert t is None or (t.dtype == x.dtype and t.shape == x.shape)
+    check(lib().rmlk_hip_rmsnorm_quantize_rows(_stream(), storage_of(x), rows, cols, _ptr(x), _ptr(add), _ptr(gamma),
+                                               float(eps), _ptr(sum_out), q.data_ptr(), _rows(q, q.shape[1]),
+                                               _ptr(scale)), "rmlk_hip_rmsnorm_quantize_rows")
+
+
+def matmul_int8_workspace_size(m: int, n: int, k: int) -> int:
+    return int(lib().rmlk_hip_matmul_int8_workspace_size(m, n, k))
+
+
+def matmul_int8(a, a_scale, wt, w_scale, out, k: int, residual=None, workspace=None) -> None:
+    """out[m, n] = (a[:, :k] . wt[:, :k]^T) * a_scale[:, None] * w_scale[None, :] (+ residual: [m, n], or [n] for
+    a bias), a int8 [m, ld] and wt int8 [n, ld] as quantize_rows leaves them."""
+    m, n = out.shape
+    _here(a, a_scale, wt, w_scale, residual, workspace)
+    assert a.dtype == wt.dtype == torch.int8 and a.shape[0] == m and wt.shape[0] == n
+    assert 0 <= k <= min(a.shape[1], wt.shape[1])
+    assert a_scale.dtype == w_scale.dtype == torch.float32 and a_scale.numel() == m and w_scale.numel() == n
+    ldr = 0
+    if residual is not None:
+        assert residual.dtype == out.dtype and residual.shape in ((m, n), (n,))
+        ldr = _rows(residual, n) if residual.dim() == 2 else 0
+        assert residual.dim() == 2 or residual.is_contiguous()
+    need = matmul_int8_workspace_size(m, n, k)
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(lib().rmlk_hip_matmul_int8(_stream(), storage_of(out), m, n, k, a.data_ptr(), _rows(a, a.shape[1]),
+                                     _ptr(a_scale), wt.data_ptr(), _rows(wt, wt.shape[1]), _ptr(w_scale),
+                                     residual.data_ptr() if residual is not None else 0, ldr, _ptr(workspace),
+                                     ws_bytes, out.data_ptr(), _rows(out, n)), "rmlk_hip_matmul_int8")
+
+
+class PagedCache:
+    """An int8 cache in pages (struct rmlk_paged_cache): k [pages, kv_heads, page_size, head_dim], v [pages, kv_heads,
+    head_dim, page_size], one float scale per page and head for each. The tensors stay the caller's."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        from ._lib import PagedCacheStruct
+        pages, kv_heads, page_size, head_dim = k.shape
+        assert k.dtype == v.dtype == torch.int8 and k_scale.dtype == v_scale.dtype == torch.float32
+        assert tuple(v.shape) == (pages, kv_heads, head_dim, page_size)
+        assert tuple(k_scale.shape) == tuple(v_scale.shape) == (pages, kv_heads)
+        assert k.device == v.device == k_scale.device == v_scale.device
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.struct = PagedCacheStruct(pages, page_size, kv_heads, head_dim, _ptr(k), _ptr(v), _ptr(k_scale),
+                                       _ptr(v_scale))
+
+    @classmethod
+    def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "PagedCache":
+        return cls(torch.empty(pages, kv_heads, page_size, head_dim, dtype=torch.int8, device=device),
+                   torch.empty(pages, kv_heads, head_dim, page_size, dtype=torch.int8, device=device),
+                   torch.empty(pages, kv_heads, device=device), torch.empty(pages, kv_heads, device=device))
+
+
+class PagedBatch:
+    """The ragged sequences of one call over a PagedCache (struct rmlk_paged_batch): first [seqs + 1], length
+    [seqs] and page_table [seqs, pages], int32 on the device; rows first[s]:first[s + 1] are the newest tokens
+    of sequence s, which then holds length[s]. tokens: the rows q, k, v and out hold; max_new and max_len:
+    bounds on a sequence's rows and length."""
+
+    def __init__(self, first, length, page_table, tokens: int, max_new: int, max_len: int):
+        from ._lib import PagedBatchStruct
+        assert first.dtype == length.dtype == page_table.dtype == torch.int32
+        seqs = length.numel()
+        assert first.numel() == seqs + 1 and page_table.dim() == 2 and page_table.shape[0] == seqs
+        assert first.device == length.device == page_table.device
+        self.first, self.length, self.page_table, self.tokens = first, length, page_table, tokens
+        self.struct = PagedBatchStruct(seqs, tokens, max_new, max_len, page_table.shape[1], _ptr(first), _ptr(length),
+                                       _ptr(page_table))
+
+
+def paged_append(cache: PagedCache, batch: PagedBatch, k, v, cos=None, sin=None, q=None, q_out=None,
+                 err_flag=None) -> None:
+    """Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated by row `position` of cos and sin (float
+    [positions, head_dim]; None: as it is); q [tokens, heads, head_dim] is rotated alike into q_out."""
+    _here(cache.k, batch.first, cos, sin, q_out, err_flag)
+    width = cache.kv_heads * cache.head_dim
+    assert k.dtype == v.dtype and k.shape[0] == v.shape[0] == batch.tokens
+    heads = 0
+    if q is not None:
+        heads = q.shape[1]
+        assert q.dtype == q_out.dtype == k.dtype and q.shape == q_out.shape == (batch.tokens, heads, cache.head_dim)
+    for t in (cos, sin):
+        assert t is None or (t.dtype == torch.float32 and t.dim() == 2 and t.shape == (cos.shape[0], cache.head_dim))
+    check(lib().rmlk_hip_paged_append(_stream(), storage_of(k), cache.struct, batch.struct, k.data_ptr(),
+                                      _rows(k, width), v.data_ptr(), _rows(v, width), _ptr(cos), _ptr(sin),
+                                      cos.shape[0] if cos is not None else 0, heads,
+                                      q.data_ptr() if q is not None else 0,
+                                      _rows(q, heads * cache.head_dim) if q is not None else 0, _ptr(q_out),
+                                      _ptr(err_flag)), "rmlk_hip_paged_append")
+
+
+def paged_attention_workspace_size(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype, heads: int) -> int:
+    dt = BFLOAT16 if dtype == torch.bfloat16 else TORCH_TO_DTYPE[dtype]
+    return int(lib().rmlk_hip_paged_attention_workspace_size(dt, cache.struct, batch.struct, heads))
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, scale: float, scale_is_mul: bool = False,
+                    workspace=None, err_flag=None) -> None:
+    """out [tokens, heads, head_dim] = causal attention of q over the cached tokens of its sequences; the rows of q
+    may lie apart (a slice of a joint projection)."""
+    heads = q.shape[1]
+    _here(cache.k, batch.first, out, workspace, err_flag)
+    assert q.dtype == out.dtype and q.shape == out.shape == (batch.tokens, heads, cache.head_dim)
+    need = paged_attention_workspace_size(cache, batch, q.dtype, heads)
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(lib().rmlk_hip_paged_attention(_stream(), storage_of(q), cache.struct, batch.struct, heads, q.data_ptr(),
+                                         _rows(q, heads * cache.head_dim), int(scale_is_mul), float(scale),
+                                         _ptr(workspace), ws_bytes, _ptr(out), _ptr(err_flag)),
+          "rmlk_hip_paged_attention")
 
 
 def memcpy_dtod_many(dsts, srcs) -> None:
