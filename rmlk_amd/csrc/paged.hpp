@@ -102,8 +102,9 @@ inline int32_t paged_args(const rmlk_paged_cache *cache, const rmlk_paged_batch 
 inline int32_t paged_pointers(const rmlk_paged_cache *cache, const rmlk_paged_batch *batch) {
     if (!batch->first || !batch->length) return RMLK_ERR_NULL_POINTER;
     if (batch->table_stride > 0 && !batch->page_table) return RMLK_ERR_NULL_POINTER;
-    if (cache->pages > 0 && (!cache->k || !cache->v || !cache->k_scale || !cache->v_scale))
+    if ((!cache->k || !cache->v || !cache->k_scale || !cache->v_scale) && cache->pages > 0)
         return RMLK_ERR_NULL_POINTER;
+    if (cache->pages == 0) return RMLK_ERR_INVALID_ARGUMENT;    // nowhere to read from, nowhere to write to
     if (!aligned16(cache->k) || !aligned16(cache->v)) return RMLK_ERR_UNSUPPORTED;
     return RMLK_OK;
 }
@@ -142,6 +143,16 @@ __device__ __forceinline__ int sequence_of(const PagedArgs &g, int piece, int un
     for (int base = 0; base < g.seqs; base += kWave) {
         const int i = base + static_cast<int>(threadIdx.x % kWave);
         s += __popcll(__ballot(i < g.seqs && g.first[i] / unit + extra * i <= piece));
+    }
+    return s;
+}
+
+// The same over rep rows of a matrix per row of the call: tile number `piece` of `unit` matrix rows.
+__device__ __forceinline__ int sequence_of_rows(const PagedArgs &g, int piece, int rep, int unit) {
+    int s = -1;
+    for (int base = 0; base < g.seqs; base += kWave) {
+        const int i = base + static_cast<int>(threadIdx.x % kWave);
+        s += __popcll(__ballot(i < g.seqs && g.first[i] * rep / unit + i <= piece));
     }
     return s;
 }

@@ -1,5 +1,29 @@
 // Attention over the paged int8 cache: out = Softmax(q . K^T * scale) . V per sequence, a query seeing the
-// tokens up to its own position.
+// tokens up to its own position; prompts, chunks of prompts and single tokens alike.
+//
+// The rows of one KV head (its rep query heads times the sequence's new tokens) form one matrix. A
+// block takes 16 * NT of them; its wavefronts share them and deal the keys out among themselves in
+// tiles of 64, each with its own running maximum, sum and output, which meet in LDS at the end. Long
+// caches are split over several blocks besides, whose normalised results a second kernel joins.
+//
+// Everything is computed transposed, so that a query stays in one lane column from its scores to its
+// output: S^T = K . Q^T by v_mfma_f32_16x16x32_f16 leaves four keys of a query in a lane, and the keys
+// of a tile are assigned to the rows of the four S^T blocks such that a lane's sixteen weights belong to
+// sixteen CONSECUTIVE tokens (16 g .. 16 g + 15 for lane group g): they are the B operand of
+// O^T += V^T . P^T as they are, and the A operand is sixteen consecutive bytes of a row of the transposed
+// V block. No score, weight or cache value passes through LDS; K and V go from memory to registers in
+// 16-byte loads, one tile ahead.
+//
+// int8 -> half: a byte b with its sign bit flipped, u = b + 128, under the high byte 0x64 is the half
+// 1024 + u; one packed add of -1152 gives b (K), one packed fma (1024 + u) * f - 1152 f gives b * f
+// exactly (V, f the page's step relative to the largest one met, E, which scales the output at the
+// end). So pages with different steps mix in one MFMA. K's step goes to the scores.
+//
+// A float query is the sum of two halves (hi + lo, 22 bits), scaled by a power of two so that its
+// largest element lies in [2^13, 2^14); a float weight likewise, exponentials being taken relative to
+// the maximum less 7 and allowed to grow to 2^15 before the reference point moves (rescaling is rare),
+// so weights down to 2^-18 of the largest keep 22 bits. For 16-bit types one half each: q is exact, a
+// weight is off by 2^-11 of itself at most, as the output is.
 #include <cmath>
 
 #include "paged.hpp"
@@ -7,84 +31,442 @@
 namespace rmlk {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTileKeys = 64;
+constexpr float kBase = 7.f;          // log2 of the weight of a key that scores the reference maximum
+constexpr float kMostWeight = 15.f;   // log2 of the largest weight before the reference point moves
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
 struct AttendArgs {
     PagedArgs c;
     const T *q;
     T *out;
+    float *part;         // partial outputs [splits][rows * heads][D], then (max, sum) [splits][rows * heads][2]
     int64_t q_stride;
-    int32_t heads;
+    int32_t heads, rep;
     float scale;         // of the scores, with log2(e)
+    int32_t pieces;      // row tiles the grid covers, per KV head and split
+    int32_t splits, chunk;   // tokens per split, a multiple of the tile
+    int32_t one_each;    // a sequence has at most one row tile: tile number = sequence
 };
 
-// A wavefront per (row, head): 64 keys at a time, a key per lane for the scores and a head dim (or two)
-// per lane for the output.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void attend_rows_kernel(AttendArgs<T> g) {
+// the four bytes of a word as halves 1024 + (b + 128)
+__device__ __forceinline__ void biased_halves(uint32_t w, h2 &lo, h2 &hi) {
+    const uint32_t x = w ^ 0x80808080u;
+    lo = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u));
+    hi = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u));
+}
+__device__ __forceinline__ h8 eight(h2 a, h2 b, h2 c, h2 d) {
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ h8 widen(uint32_t w0, uint32_t w1) {
+    const h2 bias = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    h2 a, b, c, d;
+    biased_halves(w0, a, b);
+    biased_halves(w1, c, d);
+    return eight(a + bias, b + bias, c + bias, d + bias);
+}
+__device__ __forceinline__ h8 widen_scaled(uint32_t w0, uint32_t w1, h2 f, h2 bias) {
+    h2 a, b, c, d;
+    biased_halves(w0, a, b);
+    biased_halves(w1, c, d);
+    return eight(__builtin_elementwise_fma(a, f, bias), __builtin_elementwise_fma(b, f, bias),
+                 __builtin_elementwise_fma(c, f, bias), __builtin_elementwise_fma(d, f, bias));
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+    v += __shfl_xor(v, 16, kWave);
+    return v + __shfl_xor(v, 32, kWave);
+}
+
+// One tile of keys on its way from memory: raw bytes of K and V, the steps of the page of the lane
+// group's tokens.
+template <int D>
+struct Tile {
+    u32x4 k[4][D / 64];
+    u32x4 v[D / 16];
+    float k_scale, v_scale;
+    bool bad;            // the page lies outside the cache
+};
+
+template <typename T, int D, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1;      // half pieces of a query value and of a weight
+    constexpr int DT = D / 16, KC = D / 64, R = 16 * NT, kPad = D + 4;
+    extern __shared__ __align__(16) float lds[];   // [WAVES][R][kPad], then (max, sum) [WAVES][R]
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int col = lane % 16, grp = lane / 16;
+
+    // Blocks of one KV head next to each other would meet on different XCDs (workgroups go round
+    // robin): the head is the fastest index, so with eight of them an XCD reads one head's cache. Last
+    // row tiles first: they see the most keys.
     if (!starts_ascend(g.c)) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(g.c);
+        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
         return;
     }
-    const int lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
-    if (item >= g.c.rows * g.heads) return;
-    const int64_t row = item / g.heads;
-    const int head = static_cast<int>(item % g.heads), kv = head / (g.heads / g.c.kv_heads);
+    const int kv = blockIdx.x % g.c.kv_heads;
+    const int rest = blockIdx.x / g.c.kv_heads;
+    const int split = rest % g.splits;
+    const int piece = g.pieces - 1 - rest / g.splits;
+    const int seq = g.one_each ? piece : sequence_of_rows(g.c, piece, g.rep, R);
+    if (seq < 0) return;
     Sequence s;
-    const int seq = sequence_of_row(g.c, row);
     if (!sequence_at(g.c, seq, s)) {
-        if (lane == 0) raise_error(g.c);
+        if (tid == 0) raise_error(g.c);
         return;
     }
-    if (row < s.row || row >= s.row + s.fresh) return;
-    const int limit = s.length - s.fresh + static_cast<int>(row - s.row) + 1;   // tokens it sees
-    const int size = 1 << g.c.page_shift;
-    const int32_t *table = g.c.table + seq * g.c.table_stride;
-    const T *q = g.q + row * g.q_stride + static_cast<int64_t>(head) * D;
-    float m = -INFINITY, sum = 0.f, acc[D / kWave] = {};
-    for (int t0 = 0; t0 < limit; t0 += kWave) {
-        const int t = t0 + lane;
-        float x = -INFINITY, vs = 0.f;
-        int64_t block = 0;
-        if (t < limit) {
-            const int32_t page = table[t >> g.c.page_shift];
-            if (page < 0 || page >= g.c.pages) {
-                raise_error(g.c);
-            } else {
-                block = static_cast<int64_t>(page) * g.c.kv_heads + kv;
-                const int8_t *k = g.c.k + (block * size + (t & (size - 1))) * D;
-                float dot = 0.f;
-                for (int d = 0; d < D; ++d) dot = fmaf(to_float(q[d]), static_cast<float>(k[d]), dot);
-                vs = g.c.v_scale[block];
-                // (a scale that is NaN, of K or of V, makes the score NaN)
-                x = dot * (g.c.k_scale[block] + 0.f * vs) * g.scale;
+    const int index = g.one_each ? 0 : piece - (s.row * g.rep / R + seq);
+    const int rows = s.fresh * g.rep, r0 = index * R;
+    if (index < 0 || r0 >= rows) return;
+    const int past = s.length - s.fresh;           // position of the sequence's first row
+    const int most = past + min(r0 + R - 1, rows - 1) / g.rep + 1;   // tokens the last row sees
+    const int least = past + r0 / g.rep + 1;
+    const int begin = split * g.chunk;
+    if (split > 0 && begin >= most) return;
+    const int end = min(most, begin + g.chunk);
+
+    // the rows of this lane column: what they see, their query as halves
+    int limit[NT];
+    float factor[NT];          // of an S^T element but for K's step
+    h8 qf[P][NT][2 * KC];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = r0 + n * 16 + col;
+        const bool live = r < rows;
+        limit[n] = live ? past + r / g.rep + 1 : 0x7fffffff;   // (a row that is not there: no mask, zeros)
+        float x[KC][16];
+        const T *src = g.q + (s.row + (live ? r / g.rep : 0)) * g.q_stride +
+                       static_cast<int64_t>(kv * g.rep + (live ? r % g.rep : 0)) * D + grp * 16;
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            load_row(src + c * 64, x[c]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (!live) x[c][i] = 0.f;
+                const uint32_t bits = __float_as_uint(x[c][i]) & 0x7fffffffu;
+                top = bits > top ? bits : top;
             }
         }
-        const bool any_nan = __any(x != x);
-        const float top = any_nan ? __uint_as_float(0x7fc00000u) : fmaxf(m, wave_max(x));
-        if (top == -INFINITY) continue;
-        const float alpha = exp2f(m - top), p = exp2f(x - top);
-        m = top;
-        sum = sum * alpha + wave_sum(p);
+        uint32_t other = __shfl_xor(top, 16, kWave);
+        top = other > top ? other : top;
+        other = __shfl_xor(top, 32, kWave);
+        top = other > top ? other : top;
+        // (an infinity or a NaN in the row: the factor is whatever, the products are NaN)
+        const int e = max(-113, static_cast<int>(top >> 23) - 127);
+        const float up = __uint_as_float(static_cast<uint32_t>(13 - e + 127) << 23);
+        factor[n] = __uint_as_float(static_cast<uint32_t>(e - 13 + 127) << 23) * g.scale;
+        if (top >= 0x7f800000u) factor[n] = __uint_as_float(0x7fc00000u);
 #pragma unroll
-        for (int i = 0; i < D / kWave; ++i) acc[i] *= alpha;
-        const int here = min(kWave, limit - t0);
-        const float pv = vs == vs ? p * vs : 0.f;
-        for (int j = 0; j < here; ++j) {
-            const float w = __shfl(pv, j, kWave);
-            const int64_t b = __shfl(static_cast<long long>(block), j, kWave);
-            const int8_t *v = g.c.v + b * size * D + ((t0 + j) & (size - 1));
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int i = 0; i < D / kWave; ++i)
-                acc[i] = fmaf(w, static_cast<float>(v[static_cast<int64_t>(i * kWave + lane) * size]), acc[i]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = x[c][h * 8 + j] * up;
+                    const _Float16 hi = static_cast<_Float16>(v);
+                    qf[0][n][c * 2 + h][j] = hi;
+                    if constexpr (P == 2) qf[1][n][c * 2 + h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
+                }
+    }
+
+    f32x4 acc[DT][NT];
+    float sum[NT], ref[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        sum[n] = 0.f;
+        ref[n] = -INFINITY;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int step_exp = -200;       // E: log2 of the largest step of V met so far
+
+    const int last_page = (s.length > 0 ? s.length - 1 : 0) >> g.c.page_shift;
+    const int size = 1 << g.c.page_shift;
+    const int32_t *table = g.c.table + seq * g.c.table_stride;
+    // pages of the tokens whose K rows (by lane column) and whose V columns (by lane group) a lane loads
+    auto pages_of = [&](int t0, int32_t &pk, int32_t &pv) {
+        pk = table[min((t0 + (col / 4) * 16) >> g.c.page_shift, last_page)];
+        pv = table[min((t0 + grp * 16) >> g.c.page_shift, last_page)];
+    };
+    auto fetch = [&](Tile<D> &t, int t0, int32_t pk, int32_t pv) {
+        t.bad = pv < 0 || pv >= g.c.pages;
+        if (t.bad) raise_error(g.c);
+        pk = pk < 0 || pk >= g.c.pages ? 0 : pk;
+        pv = t.bad ? 0 : pv;
+        const int64_t bk = (static_cast<int64_t>(pk) * g.c.kv_heads + kv), bv = static_cast<int64_t>(pv) * g.c.kv_heads + kv;
+        const int8_t *k = g.c.k + (bk * size + ((t0 + (col / 4) * 16 + col % 4) & (size - 1))) * D + grp * 16;
+        const int8_t *v = g.c.v + bv * size * D + ((t0 + grp * 16) & (size - 1)) + static_cast<int64_t>(col) * size;
+        t.k_scale = g.c.k_scale[bv];
+        t.v_scale = g.c.v_scale[bv];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) t.k[j][c] = *reinterpret_cast<const u32x4 *>(k + j * 4 * D + c * 64);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + static_cast<int64_t>(d) * 16 * size);
+    };
+    auto compute = [&](const Tile<D> &t, int t0) {
+        const bool masked = t0 + kTileKeys > least || __any(t.bad);
+        // V's steps relative to the largest; a step that is no number marks the scores instead
+        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f);
+        const float vs = odd || t.bad ? 0.f : t.v_scale;
+        int e = static_cast<int>((__float_as_uint(vs) >> 23) & 255u) - 127;
+        e = max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
+                max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
+        if (e > step_exp) {
+            const float down = ldexpf(1.f, step_exp - e);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[d][n] *= down;
+            step_exp = e;
+        }
+        const _Float16 f1 = static_cast<_Float16>(ldexpf(vs, -step_exp));
+        const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
+        const h2 vf = {f1, f1}, vbias = {b1, b1};
+        const float kc = odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale;
+        float c[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) c[n] = factor[n] * kc;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            f32x4 sc[2][NT];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < 2 * KC; ++q) {
+                    const u32x4 raw = t.k[2 * hh + j][q / 2];
+                    const h8 kf = q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[p][n][q], sc[j][n], 0, 0, 0);
+                }
+            }
+            // exponents relative to the reference point
+            const int key = t0 + grp * 16 + hh * 8;
+            auto exponents = [&](int n, float (&x)[8]) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v = fmaf(sc[j][n][i], c[n], -ref[n]);
+                        if (masked) v = key + j * 4 + i < limit[n] && !t.bad ? v : -INFINITY;
+                        x[j * 4 + i] = v;
+                        top = fmaxf(top, v);
+                    }
+                return top;
+            };
+            float x[NT][8];
+            bool beyond = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) beyond = exponents(n, x[n]) > kMostWeight || beyond;
+            if (__any(beyond)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool see = !masked || (key + j * 4 + i < limit[n] && !t.bad);
+                            top = fmaxf(top, see ? sc[j][n][i] * c[n] : -INFINITY);
+                        }
+                    const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
+                    const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
+                    ref[n] = now;
+                    sum[n] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
+                    exponents(n, x[n]);
+                }
+            }
+            h8 pf[P][NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float w = __builtin_amdgcn_exp2f(x[n][i]);
+                    sum[n] += w;
+                    const _Float16 hi = static_cast<_Float16>(w);
+                    pf[0][n][i] = hi;
+                    if constexpr (P == 2) pf[1][n][i] = static_cast<_Float16>(w - static_cast<float>(hi));
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const h8 va = widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias);
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
+            }
+        }
+    };
+
+    // tiles begin + 64 * (wave + i * WAVES): the next one is on its way while one is computed, the page
+    // numbers of the one after that besides
+    constexpr int kStride = kTileKeys * WAVES;
+    int t0 = begin + wave * kTileKeys;
+    if (t0 < end) {
+        Tile<D> one, two;
+        int32_t pk, pv;
+        pages_of(t0, pk, pv);
+        int32_t next_pk = 0, next_pv = 0;
+        if (t0 + kStride < end) pages_of(t0 + kStride, next_pk, next_pv);
+        fetch(one, t0, pk, pv);
+        while (true) {
+            auto half_step = [&](Tile<D> &now, Tile<D> &next) {
+                const int t1 = t0 + kStride, t2 = t1 + kStride;
+                const bool more = t1 < end;
+                if (more) {
+                    const int32_t a = next_pk, b = next_pv;
+                    if (t2 < end) pages_of(t2, next_pk, next_pv);
+                    fetch(next, t1, a, b);
+                }
+                compute(now, t0);
+                t0 = t1;
+                return more;
+            };
+            if (!half_step(one, two)) break;
+            if (!half_step(two, one)) break;
         }
     }
-    T *out = g.out + (row * g.heads + head) * D;
+
+    // a wavefront's own mean first (bounded by the largest |v|), then the mean of the means
+    float2 *stats = reinterpret_cast<float2 *>(lds + WAVES * R * kPad);
 #pragma unroll
-    for (int i = 0; i < D / kWave; ++i) out[i * kWave + lane] = static_cast<T>(m == -INFINITY ? 0.f : acc[i] / sum);
+    for (int n = 0; n < NT; ++n) {
+        const float total = across_groups_sum(sum[n]);
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        if (grp == 0) stats[wave * R + n * 16 + col] = float2{ref[n], total};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            f32x4 o = acc[d][n] * inv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], step_exp);
+            *reinterpret_cast<f32x4 *>(lds + (wave * R + n * 16 + col) * kPad + d * 16 + grp * 4) = o;
+        }
+    }
+    __syncthreads();
+    const int64_t all_rows = g.c.rows * g.heads;
+    for (int i = tid; i < R * (D / 4); i += WAVES * kWave) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        const int r = r0 + row;
+        if (r >= rows) break;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w * R + row].x);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float2 st = stats[w * R + row];
+            const float weight = st.y == 0.f ? 0.f : st.y * __builtin_amdgcn_exp2f(st.x - top);
+            total += weight;
+            o += *reinterpret_cast<const f32x4 *>(lds + (w * R + row) * kPad + d) * weight;
+        }
+        o *= total == 0.f ? 0.f : 1.f / total;
+        const int64_t at = (s.row + r / g.rep) * static_cast<int64_t>(g.heads) + kv * g.rep + r % g.rep;
+        if (past + r / g.rep + 1 <= g.chunk) {     // (all it sees lies in the first split)
+            if (split == 0) {
+                T *dst = g.out + at * D + d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[e] = static_cast<T>(o[e]);
+            }
+        } else {
+            *reinterpret_cast<f32x4 *>(g.part + (split * all_rows + at) * D + d) = o;
+            if (d == 0)
+                reinterpret_cast<float2 *>(g.part + g.splits * all_rows * D)[split * all_rows + at] = float2{top, total};
+        }
+    }
+}
+
+// The splits of the rows that see more than one: a wavefront per (row, head).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
+    if (!starts_ascend(g.c)) return;
+    const int lane = threadIdx.x % kWave;
+    const int64_t all_rows = g.c.rows * g.heads;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (at >= all_rows) return;
+    const int64_t row = at / g.heads;
+    Sequence s;
+    if (!sequence_at(g.c, sequence_of_row(g.c, row), s) || row < s.row || row >= s.row + s.fresh) return;
+    const int limit = s.length - s.fresh + static_cast<int>(row - s.row) + 1;
+    if (limit <= g.chunk) return;
+    const int parts = (limit + g.chunk - 1) / g.chunk;
+    const float2 *stats = reinterpret_cast<const float2 *>(g.part + g.splits * all_rows * D) + at;
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += kWave) top = fmaxf(top, stats[i * all_rows].x);
+    top = wave_max(top);
+    constexpr int N = D / kWave;
+    float o[N] = {}, total = 0.f;
+    for (int i = 0; i < parts; ++i) {
+        const float2 st = stats[i * all_rows];
+        const float weight = st.y == 0.f ? 0.f : st.y * __builtin_amdgcn_exp2f(st.x - top);
+        total += weight;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fmaf(g.part[(i * all_rows + at) * D + lane * N + e], weight, o[e]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < N; ++e) g.out[at * D + lane * N + e] = static_cast<T>(o[e] * inv);
+}
+
+// How a call is cut: rows per block, tiles of rows, splits of the keys.
+struct Plan {
+    int nt;
+    int64_t pieces;
+    int32_t splits, chunk;
+    bool one_each;
+    size_t workspace;
+};
+constexpr int kWaves = 4;
+
+Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
+    Plan p{};
+    const int64_t rep = heads / c.kv_heads, rows = c.max_new * rep;
+    p.nt = rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
+    const int64_t tile = 16 * p.nt;
+    p.one_each = rows <= tile;
+    p.pieces = p.one_each ? c.seqs : c.rows * rep / tile + c.seqs;
+    const int64_t step = kTileKeys * kWaves;
+    const int64_t len = c.max_length > 0 ? c.max_length : 1;
+    const int64_t blocks = p.pieces * c.kv_heads;
+    int64_t splits = (2 * kNumCU + blocks - 1) / blocks;
+    if (p.nt == 1 && splits < (len + 4095) / 4096) splits = (len + 4095) / 4096;
+    const int64_t most = (len + step - 1) / step;
+    splits = splits < most ? splits : most;
+    splits = splits < 64 ? splits : 64;
+    const int64_t chunk = ((len + splits - 1) / splits + step - 1) / step * step;
+    p.chunk = static_cast<int32_t>(chunk);
+    p.splits = static_cast<int32_t>((len + chunk - 1) / chunk);
+    p.workspace = p.splits > 1 ? static_cast<size_t>(p.splits) * c.rows * heads * (head_dim + 2) * sizeof(float) : 0;
+    return p;
+}
+
+template <typename T, int D, int NT>
+int32_t launch_attend(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
+    constexpr int lds = kWaves * 16 * NT * ((D + 4) * 4 + 8);
+    auto kern = attend_kernel<T, D, NT, kWaves>;
+    static DynamicLdsGrant grant;
+    if (const int32_t bad = grant.ensure(kern, lds); bad != RMLK_OK) return bad;
+    kern<<<static_cast<uint32_t>(blocks), kWaves * kWave, lds, st>>>(g);
+    return launch_status();
 }
 
 int32_t attend_checks(int32_t dtype, const rmlk_paged_cache *cache, const rmlk_paged_batch *batch, int64_t heads,
@@ -107,8 +489,8 @@ extern "C" {
 size_t rmlk_hip_paged_attention_workspace_size(int32_t dtype, const rmlk_paged_cache *cache,
                                                const rmlk_paged_batch *batch, int64_t heads) {
     PagedArgs c{};
-    if (attend_checks(dtype, cache, batch, heads, nullptr, &c) != RMLK_OK) return 0;
-    return 0;
+    if (attend_checks(dtype, cache, batch, heads, nullptr, &c) != RMLK_OK || c.seqs == 0 || c.rows == 0) return 0;
+    return plan_for(c, dtype, cache->head_dim, heads).workspace;
 }
 
 int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk_paged_cache *cache,
@@ -125,19 +507,41 @@ int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk
     const int64_t unit = dtype == RMLK_FLOAT ? 4 : 8;
     if (q_stride < heads * d) return RMLK_ERR_SIZE_MISMATCH;
     if (q_stride % unit || !aligned16(q) || !aligned16(out)) return RMLK_ERR_UNSUPPORTED;
-    const int64_t blocks = (c.rows * heads + 3) / 4;
-    if (blocks > (1 << 23)) return RMLK_ERR_TOO_LARGE;
+    const Plan plan = plan_for(c, dtype, d, heads);
+    const int64_t blocks = plan.pieces * c.kv_heads * plan.splits;
+    const int64_t join_blocks = (c.rows * heads + 3) / 4;
+    if (blocks > (1 << 23) || join_blocks > (1 << 23) || c.rows * heads > 0x3fffffff) return RMLK_ERR_TOO_LARGE;
+    if (plan.workspace > 0) {
+        if (!workspace) return RMLK_ERR_NULL_POINTER;
+        if (!aligned16(workspace)) return RMLK_ERR_UNSUPPORTED;
+        if (workspace_bytes < plan.workspace) return RMLK_ERR_WORKSPACE;
+    }
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
         AttendArgs<T> g{};
         g.c = c;
         g.q = static_cast<const T *>(q);
         g.out = static_cast<T *>(out);
+        g.part = static_cast<float *>(workspace);
         g.q_stride = q_stride;
         g.heads = static_cast<int32_t>(heads);
+        g.rep = static_cast<int32_t>(heads / c.kv_heads);
         g.scale = (scale_is_mul ? scale : 1.f / scale) * kLog2e;
-        if (d == 64) attend_rows_kernel<T, 64><<<static_cast<uint32_t>(blocks), kThreads, 0, st>>>(g);
-        else attend_rows_kernel<T, 128><<<static_cast<uint32_t>(blocks), kThreads, 0, st>>>(g);
+        g.pieces = static_cast<int32_t>(plan.pieces);
+        g.splits = plan.splits;
+        g.chunk = plan.chunk;
+        g.one_each = plan.one_each;
+        int32_t bad;
+        if (d == 64) {
+            bad = plan.nt == 1   ? launch_attend<T, 64, 1>(st, g, blocks)
+                  : plan.nt == 2 ? launch_attend<T, 64, 2>(st, g, blocks)
+                                 : launch_attend<T, 64, 4>(st, g, blocks);
+        } else {
+            bad = plan.nt == 1 ? launch_attend<T, 128, 1>(st, g, blocks) : launch_attend<T, 128, 2>(st, g, blocks);
+        }
+        if (bad != RMLK_OK || plan.splits == 1) return bad;
+        if (d == 64) attend_join_kernel<T, 64><<<static_cast<uint32_t>(join_blocks), 256, 0, st>>>(g);
+        else attend_join_kernel<T, 128><<<static_cast<uint32_t>(join_blocks), 256, 0, st>>>(g);
         return launch_status();
     });
 }
