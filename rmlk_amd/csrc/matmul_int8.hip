@@ -1,12 +1,17 @@
 // c[m, n] = (a . wt^T) * a_scale[row] * w_scale[column] (+ residual), a and wt int8 (K-contiguous).
 // The integer sums are exact in 32 bits (k < 2^17, |values| <= 128), whatever their order; the
 // epilogue scales them in float and rounds once to the output type.
+//
+// Two kernels. Up to 64 rows the weights are what is read, once: a block takes 16 channels and all the
+// rows, its wavefronts deal K out among themselves and meet in LDS (int8_few_rows_kernel). Beyond, tiles
+// of a and wt go through LDS (int8_tiles_kernel).
 #include "paged.hpp"
 
 namespace rmlk {
 namespace {
 
-constexpr int kThreads = 256;
+typedef int32_t v4i __attribute__((ext_vector_type(4)));
+typedef int32_t v16i __attribute__((ext_vector_type(16)));
 
 template <typename T>
 struct Int8Args {
@@ -18,16 +23,17 @@ struct Int8Args {
     T *c;
     int64_t lda, ldw, ldr, ldc;
     int32_t m, n, k;
+    int32_t tiles_m, tiles_n;
 };
 
 template <typename T>
-__device__ __forceinline__ void store_scaled(const Int8Args<T> &g, int row, int col, int32_t sum) {
-    float v = static_cast<float>(sum) * g.a_scale[row] * g.w_scale[col];
+__device__ __forceinline__ void store_scaled(const Int8Args<T> &g, int row, int col, int32_t sum, float sa, float sw) {
+    float v = static_cast<float>(sum) * sa * sw;
     if (g.residual) v += to_float(g.residual[row * g.ldr + col]);
     g.c[row * g.ldc + col] = static_cast<T>(v);
 }
 
-// bytes k .. of a 16-byte unit cleared
+// bytes `valid` .. of a 16-byte unit cleared (valid may be negative or beyond 16)
 __device__ __forceinline__ u32x4 clear_tail(u32x4 v, int valid) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -37,21 +43,297 @@ __device__ __forceinline__ u32x4 clear_tail(u32x4 v, int valid) {
     return v;
 }
 
-// A thread per output.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void int8_outputs_kernel(Int8Args<T> g) {
-    const int col = blockIdx.x * 64 + threadIdx.x % 64;
-    const int row = blockIdx.y * 4 + threadIdx.x / 64;
-    if (row >= g.m || col >= g.n) return;
-    const int8_t *a = g.a + row * g.lda, *w = g.w + col * g.ldw;
-    int32_t sum = 0;
-    for (int k0 = 0; k0 < g.k; k0 += 16) {
-        const u32x4 av = clear_tail(*reinterpret_cast<const u32x4 *>(a + k0), g.k - k0);
-        const u32x4 wv = *reinterpret_cast<const u32x4 *>(w + k0);
+// 16 channels x 16 * MT rows per block, v_mfma_i32_16x16x64_i8 with the channels as its rows: lane (l % 16,
+// l / 16) holds 16 consecutive bytes of channel l % 16, and of row l % 16 of a, straight from memory. A
+// wavefront takes every WAVES-th run of 256 bytes of K. Bytes of a behind k are cleared, so what the
+// weights hold there does not matter; units behind k are read from the row's start instead.
+template <typename T, int MT, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void int8_few_rows_kernel(Int8Args<T> g) {
+    __shared__ int32_t parts[WAVES][MT][kWave][4];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int n0 = blockIdx.x * 16;
+    const int8_t *w = g.w + static_cast<int64_t>(min(n0 + lane % 16, g.n - 1)) * g.ldw;
+    const int8_t *a[MT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_sdot4(av[i], wv[i], sum, false);
+    for (int t = 0; t < MT; ++t) a[t] = g.a + static_cast<int64_t>(min(t * 16 + lane % 16, g.m - 1)) * g.lda;
+    v4i acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = v4i{0, 0, 0, 0};
+    for (int k0 = wave * 256; k0 < g.k; k0 += WAVES * 256) {
+        u32x4 wv[4], av[4][MT];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = k0 + j * 64 + lane / 16 * 16;
+            wv[j] = *reinterpret_cast<const u32x4 *>(w + (at < g.k ? at : 0));
+#pragma unroll
+            for (int t = 0; t < MT; ++t) av[j][t] = *reinterpret_cast<const u32x4 *>(a[t] + (at < g.k ? at : 0));
+        }
+        if (k0 + 256 > g.k) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) av[j][t] = clear_tail(av[j][t], g.k - (k0 + j * 64 + lane / 16 * 16));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, wv[j]),
+                                                               __builtin_bit_cast(v4i, av[j][t]), acc[t], 0, 0, 0);
     }
-    store_scaled(g, row, col, sum);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) *reinterpret_cast<v4i *>(parts[wave][t][lane]) = acc[t];
+    __syncthreads();
+    for (int i = tid; i < MT * 256; i += WAVES * kWave) {
+        const int row = i / 16, col = i % 16;        // outputs of a row next to each other
+        if (row >= g.m || n0 + col >= g.n) continue;
+        // C layout: lane (row % 16) + 16 * (channel / 4), register channel % 4
+        int32_t sum = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) sum += parts[v][row / 16][row % 16 + col / 4 * 16][col % 4];
+        store_scaled(g, row, n0 + col, sum, g.a_scale[row], g.w_scale[n0 + col]);
+    }
+}
+
+// Block tile (32 TM WM) x (32 TN WN), WM x WN wavefronts of 32 TM x 32 TN, K steps of 64 bytes.
+// LDS rows are 64 bytes (four 16-byte units), unpadded - a direct load writes 64 lanes x 16 bytes as one
+// contiguous KiB, sixteen rows - and unit u of row r lives at position u ^ ((r >> 2) & 3) of its row, so
+// that the sixteen lanes a 128-bit fragment read serves together cover all banks once. STAGES stages: the
+// stage for K step s + STAGES - 1 is requested during step s into the one read in step s - 1; loads
+// complete in order, so vmcnt tells when the next stage is there; one barrier per K step, a quarter into
+// its second half, behind which the first fragments of the next step are read. LDS reads and direct
+// loads are dealt out between the MFMAs. Rows behind m and n are read from the last row and not stored.
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g) {
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 64;
+    constexpr int kAStage = BM * BK, kStage = (BM + BN) * BK;
+    constexpr int A_LOADS = BM / 16 / NW, B_LOADS = BN / 16 / NW, kLoads = A_LOADS + B_LOADS;
+    extern __shared__ __align__(16) unsigned char smem[];
+
+    // Tiles in groups of GM x GN that an XCD works on at a time (workgroups go to the XCDs round robin),
+    // so that its L2 fetches each row of a group once.
+    const int total = g.tiles_m * g.tiles_n, per_xcd = (total + 7) / 8;
+    const int t = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+    if (static_cast<int>(blockIdx.x / 8) >= per_xcd || t >= total) return;
+    constexpr int GM = 8;
+    const int group = t / (GM * g.tiles_n), first_m = group * GM;
+    const int gm = min(GM, g.tiles_m - first_m);
+    const int in_group = t - group * GM * g.tiles_n;
+    const int tile_m = first_m + in_group % gm, tile_n = in_group / gm;
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int n_steps = g.k / BK;
+
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int wm = wave / WN, wn = wave % WN;
+    const int l32 = lane % 32, half = lane / 32;
+
+    const int src_row = lane / 4, src_unit = (lane % 4) ^ ((lane / 16) & 3);
+    uint32_t a_voff[A_LOADS], b_voff[B_LOADS];
+#pragma unroll
+    for (int j = 0; j < A_LOADS; ++j) {
+        const int row = min((wave + NW * j) * 16 + src_row, g.m - 1 - m0);
+        a_voff[j] = static_cast<uint32_t>(row * g.lda + src_unit * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < B_LOADS; ++j) {
+        const int row = min((wave + NW * j) * 16 + src_row, g.n - 1 - n0);
+        b_voff[j] = static_cast<uint32_t>(row * g.ldw + src_unit * 16);
+    }
+    const int8_t *a_ptr = g.a + static_cast<int64_t>(m0) * g.lda;
+    const int8_t *b_ptr = g.w + static_cast<int64_t>(n0) * g.ldw;
+    const uint32_t lds0 =
+        __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + wave * 1024u);
+
+    auto direct_load = [&](uint32_t lds_addr, const int8_t *base, uint32_t voff) {
+        // (one wait state between a scalar write of M0 and the LDS-bound load that reads it)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(lds_addr), "v"(voff), "s"(base)
+                     : "memory", "m0");
+    };
+    auto load_op = [&](int buf, auto o_tag) {
+        constexpr int o = decltype(o_tag)::value;
+        const uint32_t base = lds0 + static_cast<uint32_t>(buf * kStage);
+        if constexpr (o < A_LOADS) direct_load(base + o * NW * 1024, a_ptr, a_voff[o]);
+        else direct_load(base + kAStage + (o - A_LOADS) * NW * 1024, b_ptr, b_voff[o - A_LOADS]);
+    };
+    auto load_stage = [&](int buf) {
+        static_for<kLoads>([&](auto o_tag) { load_op(buf, o_tag); });
+        a_ptr += BK;
+        b_ptr += BK;
+    };
+
+    int frag_off[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) frag_off[c] = l32 * 64 + ((c * 2 + half) ^ ((l32 / 4) & 3)) * 16;
+    const int a_base = wm * TM * 2048, b_base = kAStage + wn * TN * 2048;
+    u32x4 af[2][TM], bf[2][TN];
+    constexpr int kFragOps = TM + TN;
+    auto frag_op = [&](int buf, int c, auto s_tag, auto o_tag) {
+        constexpr int s = decltype(s_tag)::value, o = decltype(o_tag)::value;
+        const unsigned char *st = smem + buf * kStage;
+        if constexpr (o < TN) bf[s][o] = *reinterpret_cast<const u32x4 *>(st + b_base + o * 2048 + frag_off[c]);
+        else af[s][o - TN] = *reinterpret_cast<const u32x4 *>(st + a_base + (o - TN) * 2048 + frag_off[c]);
+    };
+
+    v16i acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+    constexpr int NM = TM * TN;
+    auto mfma_at = [&](auto s_tag, auto q_tag) {
+        constexpr int s = decltype(s_tag)::value, q = decltype(q_tag)::value, i = q / TN, j = q % TN;
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(v4i, af[s][i]),
+                                                          __builtin_bit_cast(v4i, bf[s][j]), acc[i][j], 0, 0, 0);
+    };
+    using Slot0 = std::integral_constant<int, 0>;
+    using Slot1 = std::integral_constant<int, 1>;
+    constexpr int kBarrierAt = NM / 4;
+    auto k_step = [&](int buf, int next, int fill, auto load_tag, auto more_tag) {
+        constexpr bool LOAD = decltype(load_tag)::value, MORE = decltype(more_tag)::value;
+        constexpr int n_loads = LOAD ? kLoads : 0;
+        static_for<NM>([&](auto q_tag) {
+            constexpr int q = decltype(q_tag)::value;
+            mfma_at(Slot0{}, q_tag);
+            static_for<kFragOps>([&](auto o_tag) {
+                constexpr int o = decltype(o_tag)::value;
+                if constexpr (o * NM / kFragOps == q) frag_op(buf, 1, Slot1{}, o_tag);
+            });
+            static_for<n_loads>([&](auto o_tag) {
+                constexpr int o = decltype(o_tag)::value;
+                if constexpr (o * NM / (n_loads > 0 ? n_loads : 1) == q) load_op(fill, o_tag);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (LOAD) {
+            a_ptr += BK;
+            b_ptr += BK;
+        }
+        constexpr int room = NM - kBarrierAt - 1;
+        static_for<NM>([&](auto q_tag) {
+            constexpr int q = decltype(q_tag)::value;
+            mfma_at(Slot1{}, q_tag);
+            if constexpr (MORE && q == kBarrierAt) {
+                // this wavefront has read all of this stage and its part of the next stage has landed;
+                // then the block meets
+                if constexpr (LOAD)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                asm volatile("s_barrier" ::: "memory");
+            }
+            if constexpr (MORE) {
+                static_for<kFragOps>([&](auto o_tag) {
+                    constexpr int o = decltype(o_tag)::value;
+                    if constexpr (kBarrierAt + 1 + (kFragOps <= room ? o : o * room / kFragOps) == q)
+                        frag_op(next, 0, Slot0{}, o_tag);
+                });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+
+    if (n_steps > 0) {
+        const int pre = n_steps < STAGES - 1 ? n_steps : STAGES - 1;
+        for (int s = 0; s < pre; ++s) load_stage(s);
+        if (pre == STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+        static_for<kFragOps>([&](auto o_tag) { frag_op(0, 0, Slot0{}, o_tag); });
+        int buf = 0, fill = STAGES - 1, step = 0;
+        auto after = [](int stage) { return stage + 1 == STAGES ? 0 : stage + 1; };
+        for (; step + STAGES - 1 < n_steps; ++step) {
+            k_step(buf, after(buf), fill, std::true_type{}, std::true_type{});
+            buf = after(buf);
+            fill = after(fill);
+        }
+        for (; step + 1 < n_steps; ++step) {
+            k_step(buf, after(buf), fill, std::false_type{}, std::true_type{});
+            buf = after(buf);
+        }
+        k_step(buf, 0, fill, std::false_type{}, std::false_type{});
+    }
+    if (g.k % BK != 0) {
+        // the rest of K, through registers: what lies behind k is zero in a
+        __syncthreads();
+        const int left = g.k - n_steps * BK - src_unit * 16;     // bytes from this lane's unit on
+        const int64_t at = static_cast<int64_t>(n_steps) * BK;
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < A_LOADS; ++j) {
+            u32x4 v = zero;
+            if (left > 0)
+                v = clear_tail(*reinterpret_cast<const u32x4 *>(g.a + static_cast<int64_t>(m0) * g.lda + at + a_voff[j]), left);
+            *reinterpret_cast<u32x4 *>(smem + (wave + NW * j) * 1024 + lane * 16) = v;
+        }
+#pragma unroll
+        for (int j = 0; j < B_LOADS; ++j) {
+            u32x4 v = zero;
+            if (left > 0) v = *reinterpret_cast<const u32x4 *>(g.w + static_cast<int64_t>(n0) * g.ldw + at + b_voff[j]);
+            *reinterpret_cast<u32x4 *>(smem + kAStage + (wave + NW * j) * 1024 + lane * 16) = v;
+        }
+        __syncthreads();
+        static_for<kFragOps>([&](auto o_tag) {
+            frag_op(0, 0, Slot0{}, o_tag);
+            frag_op(0, 1, Slot1{}, o_tag);
+        });
+        static_for<NM>([&](auto q_tag) {
+            mfma_at(Slot0{}, q_tag);
+            mfma_at(Slot1{}, q_tag);
+        });
+    }
+
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int col = n0 + (wn * TN + j) * 32 + l32;
+        if (col >= g.n) continue;
+        const float sw = g.w_scale[col];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = m0 + (wm * TM + i) * 32 + 8 * (r / 4) + 4 * half + (r % 4);
+                if (row < g.m) store_scaled(g, row, col, acc[i][j][r], g.a_scale[row], sw);
+            }
+    }
+}
+
+template <typename T, int MT, int WAVES>
+int32_t launch_few_rows(hipStream_t st, const Int8Args<T> &g) {
+    int8_few_rows_kernel<T, MT, WAVES><<<static_cast<uint32_t>((g.n + 15) / 16), WAVES * kWave, 0, st>>>(g);
+    return launch_status();
+}
+
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+int32_t launch_tiles(hipStream_t st, Int8Args<T> g) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, lds = STAGES * (BM + BN) * 64;
+    static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+    g.tiles_m = (g.m + BM - 1) / BM;
+    g.tiles_n = (g.n + BN - 1) / BN;
+    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
+    if (tiles > (1 << 21)) return RMLK_ERR_TOO_LARGE;
+    auto kern = int8_tiles_kernel<T, TM, TN, WM, WN, STAGES>;
+    static DynamicLdsGrant grant;
+    if (const int32_t bad = grant.ensure(kern, lds); bad != RMLK_OK) return bad;
+    kern<<<static_cast<uint32_t>((tiles + 7) / 8 * 8), WM * WN * kWave, lds, st>>>(g);
+    return launch_status();
+}
+
+template <typename T>
+int32_t launch_int8(hipStream_t st, const Int8Args<T> &g) {
+    if (g.m <= 64) {
+        const bool wide = static_cast<int64_t>(g.n) >= 16 * 2 * kNumCU;   // blocks enough for every unit
+        if (g.m <= 16) return wide ? launch_few_rows<T, 1, 8>(st, g) : launch_few_rows<T, 1, 16>(st, g);
+        if (g.m <= 32) return launch_few_rows<T, 2, 8>(st, g);
+        return launch_few_rows<T, 4, 8>(st, g);
+    }
+    const int64_t big = static_cast<int64_t>((g.m + 255) / 256) * ((g.n + 255) / 256);
+    if (big >= kNumCU * 3 / 4) return launch_tiles<T, 4, 2, 2, 4, 4>(st, g);
+    return launch_tiles<T, 2, 2, 2, 2, 4>(st, g);
 }
 
 }  // namespace
@@ -73,7 +355,7 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
     if (m == 0 || n == 0) return RMLK_OK;
     if ((k > 0 && (!a || !wt)) || !a_scale || !w_scale || !c) return RMLK_ERR_NULL_POINTER;
     if (lda < k || ldw < k || ldc < n || (residual && ldr != 0 && ldr < n)) return RMLK_ERR_SIZE_MISMATCH;
-    if (k >= 131072 || m > 0xffff * 4 || n > 0x3fffffff) return RMLK_ERR_TOO_LARGE;
+    if (k >= 131072 || m > 0x3fffffff || n > 0x3fffffff || lda >= (1 << 23) || ldw >= (1 << 23)) return RMLK_ERR_TOO_LARGE;
     if (lda % 16 != 0 || ldw % 16 != 0 || !aligned16(a) || !aligned16(wt)) return RMLK_ERR_UNSUPPORTED;
     const size_t need = rmlk_hip_matmul_int8_workspace_size(m, n, k);
     if (need > 0) {
@@ -96,9 +378,7 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
         g.m = static_cast<int32_t>(m);
         g.n = static_cast<int32_t>(n);
         g.k = static_cast<int32_t>(k);
-        int8_outputs_kernel<T><<<dim3(static_cast<uint32_t>((n + 63) / 64), static_cast<uint32_t>((m + 3) / 4)),
-                                 kThreads, 0, st>>>(g);
-        return launch_status();
+        return launch_int8(st, g);
     });
 }
 
