@@ -24,6 +24,7 @@ struct Int8Args {
     int64_t lda, ldw, ldr, ldc;
     int32_t m, n, k;
     int32_t tiles_m, tiles_n;
+    int32_t wide;        // eight outputs (and residuals) of a row are whole 16-byte units
 };
 
 template <typename T>
@@ -95,19 +96,20 @@ __global__ __launch_bounds__(WAVES *kWave) void int8_few_rows_kernel(Int8Args<T>
     }
 }
 
-// Block tile (32 TM WM) x (32 TN WN), WM x WN wavefronts of 32 TM x 32 TN, K steps of 64 bytes.
-// LDS rows are 64 bytes (four 16-byte units), unpadded - a direct load writes 64 lanes x 16 bytes as one
-// contiguous KiB, sixteen rows - and unit u of row r lives at position u ^ ((r >> 2) & 3) of its row, so
-// that the sixteen lanes a 128-bit fragment read serves together cover all banks once. STAGES stages: the
-// stage for K step s + STAGES - 1 is requested during step s into the one read in step s - 1; loads
-// complete in order, so vmcnt tells when the next stage is there; one barrier per K step, a quarter into
-// its second half, behind which the first fragments of the next step are read. LDS reads and direct
-// loads are dealt out between the MFMAs. Rows behind m and n are read from the last row and not stored.
-template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+// Block tile (32 TM WM) x (32 TN WN), WM x WN wavefronts of 32 TM x 32 TN, K steps of 128 bytes: whole
+// cache lines (with steps of 64 bytes every line crossed from the L2 twice).
+// LDS rows are 128 bytes (eight 16-byte units), unpadded - a direct load writes 64 lanes x 16 bytes as one
+// contiguous KiB, eight rows - and unit u of row r lives at position u ^ ((r >> 1) & 7) of its row, so
+// that the sixteen lanes a 128-bit fragment read serves together cover all banks once. Two stages: the
+// one for K step s + 1 is requested in the first quarter of step s into the one read in step s - 1; one
+// barrier per K step, in its last quarter, behind which the first fragments of the next step are read.
+// LDS reads and direct loads are dealt out between the MFMAs. Rows behind m and n are read from the last
+// row and not stored.
+template <typename T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g) {
-    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 64;
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, CHUNKS = 4;
     constexpr int kAStage = BM * BK, kStage = (BM + BN) * BK;
-    constexpr int A_LOADS = BM / 16 / NW, B_LOADS = BN / 16 / NW, kLoads = A_LOADS + B_LOADS;
+    constexpr int A_LOADS = BM / 8 / NW, B_LOADS = BN / 8 / NW, kLoads = A_LOADS + B_LOADS;
     extern __shared__ __align__(16) unsigned char smem[];
 
     // Tiles in groups of GM x GN that an XCD works on at a time (workgroups go to the XCDs round robin),
@@ -127,17 +129,19 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     const int wm = wave / WN, wn = wave % WN;
     const int l32 = lane % 32, half = lane / 32;
 
-    const int src_row = lane / 4, src_unit = (lane % 4) ^ ((lane / 16) & 3);
+    // lane l of piece q (eight rows) fills LDS unit l of the piece: row l / 8, position l % 8
     uint32_t a_voff[A_LOADS], b_voff[B_LOADS];
+    auto piece_row = [&](int q) { return q * 8 + lane / 8; };
+    auto piece_unit = [&](int q) { return (lane % 8) ^ ((piece_row(q) >> 1) & 7); };
 #pragma unroll
     for (int j = 0; j < A_LOADS; ++j) {
-        const int row = min((wave + NW * j) * 16 + src_row, g.m - 1 - m0);
-        a_voff[j] = static_cast<uint32_t>(row * g.lda + src_unit * 16);
+        const int q = wave + NW * j;
+        a_voff[j] = static_cast<uint32_t>(min(piece_row(q), g.m - 1 - m0) * g.lda + piece_unit(q) * 16);
     }
 #pragma unroll
     for (int j = 0; j < B_LOADS; ++j) {
-        const int row = min((wave + NW * j) * 16 + src_row, g.n - 1 - n0);
-        b_voff[j] = static_cast<uint32_t>(row * g.ldw + src_unit * 16);
+        const int q = wave + NW * j;
+        b_voff[j] = static_cast<uint32_t>(min(piece_row(q), g.n - 1 - n0) * g.ldw + piece_unit(q) * 16);
     }
     const int8_t *a_ptr = g.a + static_cast<int64_t>(m0) * g.lda;
     const int8_t *b_ptr = g.w + static_cast<int64_t>(n0) * g.ldw;
@@ -163,17 +167,28 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         b_ptr += BK;
     };
 
-    int frag_off[2];
+    // LDS addresses of the fragments of every chunk, moved to the other stage at the end of a step
+    static_assert((kStage & (kStage - 1)) == 0, "stages are told apart by one address bit");
+    uint32_t a_addr[CHUNKS], b_addr[CHUNKS];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) frag_off[c] = l32 * 64 + ((c * 2 + half) ^ ((l32 / 4) & 3)) * 16;
-    const int a_base = wm * TM * 2048, b_base = kAStage + wn * TN * 2048;
+    for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t off = l32 * BK + ((c * 2 + half) ^ ((l32 >> 1) & 7)) * 16;
+        a_addr[c] = wm * TM * 32 * BK + off;
+        b_addr[c] = kAStage + wn * TN * 32 * BK + off;
+    }
     u32x4 af[2][TM], bf[2][TN];
     constexpr int kFragOps = TM + TN;
-    auto frag_op = [&](int buf, int c, auto s_tag, auto o_tag) {
+    auto frag_op = [&](int c, auto s_tag, auto o_tag) {
         constexpr int s = decltype(s_tag)::value, o = decltype(o_tag)::value;
-        const unsigned char *st = smem + buf * kStage;
-        if constexpr (o < TN) bf[s][o] = *reinterpret_cast<const u32x4 *>(st + b_base + o * 2048 + frag_off[c]);
-        else af[s][o - TN] = *reinterpret_cast<const u32x4 *>(st + a_base + (o - TN) * 2048 + frag_off[c]);
+        if constexpr (o < TN) bf[s][o] = *reinterpret_cast<const u32x4 *>(smem + b_addr[c] + o * 32 * BK);
+        else af[s][o - TN] = *reinterpret_cast<const u32x4 *>(smem + a_addr[c] + (o - TN) * 32 * BK);
+    };
+    auto other_stage = [&]() {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            a_addr[c] ^= kStage;
+            b_addr[c] ^= kStage;
+        }
     };
 
     v16i acc[TM][TN];
@@ -193,23 +208,28 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     using Slot0 = std::integral_constant<int, 0>;
     using Slot1 = std::integral_constant<int, 1>;
     constexpr int kBarrierAt = NM / 4;
-    auto k_step = [&](int buf, int next, int fill, auto load_tag, auto more_tag) {
-        constexpr bool LOAD = decltype(load_tag)::value, MORE = decltype(more_tag)::value;
-        constexpr int n_loads = LOAD ? kLoads : 0;
-        static_for<NM>([&](auto q_tag) {
-            constexpr int q = decltype(q_tag)::value;
-            mfma_at(Slot0{}, q_tag);
-            static_for<kFragOps>([&](auto o_tag) {
-                constexpr int o = decltype(o_tag)::value;
-                if constexpr (o * NM / kFragOps == q) frag_op(buf, 1, Slot1{}, o_tag);
+    auto k_step = [&](int fill, auto more_tag) {
+        constexpr bool MORE = decltype(more_tag)::value;
+        static_for<CHUNKS - 1>([&](auto c_tag) {
+            constexpr int c = decltype(c_tag)::value;
+            using Now = std::integral_constant<int, c % 2>;
+            using Next = std::integral_constant<int, (c + 1) % 2>;
+            static_for<NM>([&](auto q_tag) {
+                constexpr int q = decltype(q_tag)::value;
+                mfma_at(Now{}, q_tag);
+                static_for<kFragOps>([&](auto o_tag) {
+                    constexpr int o = decltype(o_tag)::value;
+                    if constexpr (o * NM / kFragOps == q) frag_op(c + 1, Next{}, o_tag);
+                });
+                if constexpr (MORE && c == 0)
+                    static_for<kLoads>([&](auto o_tag) {
+                        constexpr int o = decltype(o_tag)::value;
+                        if constexpr (o * NM / kLoads == q) load_op(fill, o_tag);
+                    });
+                __builtin_amdgcn_sched_barrier(0);
             });
-            static_for<n_loads>([&](auto o_tag) {
-                constexpr int o = decltype(o_tag)::value;
-                if constexpr (o * NM / (n_loads > 0 ? n_loads : 1) == q) load_op(fill, o_tag);
-            });
-            __builtin_amdgcn_sched_barrier(0);
         });
-        if constexpr (LOAD) {
+        if constexpr (MORE) {
             a_ptr += BK;
             b_ptr += BK;
         }
@@ -218,19 +238,17 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
             constexpr int q = decltype(q_tag)::value;
             mfma_at(Slot1{}, q_tag);
             if constexpr (MORE && q == kBarrierAt) {
-                // this wavefront has read all of this stage and its part of the next stage has landed;
+                // this wavefront has read all of this stage and its part of the next one has landed;
                 // then the block meets
-                if constexpr (LOAD)
-                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 asm volatile("s_barrier" ::: "memory");
+                other_stage();
             }
             if constexpr (MORE) {
                 static_for<kFragOps>([&](auto o_tag) {
                     constexpr int o = decltype(o_tag)::value;
                     if constexpr (kBarrierAt + 1 + (kFragOps <= room ? o : o * room / kFragOps) == q)
-                        frag_op(next, 0, Slot0{}, o_tag);
+                        frag_op(0, Slot0{}, o_tag);
                 });
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -238,67 +256,104 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     };
 
     if (n_steps > 0) {
-        const int pre = n_steps < STAGES - 1 ? n_steps : STAGES - 1;
-        for (int s = 0; s < pre; ++s) load_stage(s);
-        if (pre == STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kLoads) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        load_stage(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
-        static_for<kFragOps>([&](auto o_tag) { frag_op(0, 0, Slot0{}, o_tag); });
-        int buf = 0, fill = STAGES - 1, step = 0;
-        auto after = [](int stage) { return stage + 1 == STAGES ? 0 : stage + 1; };
-        for (; step + STAGES - 1 < n_steps; ++step) {
-            k_step(buf, after(buf), fill, std::true_type{}, std::true_type{});
-            buf = after(buf);
-            fill = after(fill);
+        static_for<kFragOps>([&](auto o_tag) { frag_op(0, Slot0{}, o_tag); });
+        int fill = 1;
+        for (int step = 1; step < n_steps; ++step) {
+            k_step(fill, std::true_type{});
+            fill ^= 1;
         }
-        for (; step + 1 < n_steps; ++step) {
-            k_step(buf, after(buf), fill, std::false_type{}, std::true_type{});
-            buf = after(buf);
-        }
-        k_step(buf, 0, fill, std::false_type{}, std::false_type{});
+        k_step(fill, std::false_type{});
     }
     if (g.k % BK != 0) {
         // the rest of K, through registers: what lies behind k is zero in a
         __syncthreads();
-        const int left = g.k - n_steps * BK - src_unit * 16;     // bytes from this lane's unit on
+        const int left = g.k - n_steps * BK;
+        const int stage = n_steps > 1 && n_steps % 2 == 0 ? kStage : 0;      // where the fragment addresses point
         const int64_t at = static_cast<int64_t>(n_steps) * BK;
         const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < A_LOADS; ++j) {
+            const int here = left - piece_unit(wave + NW * j) * 16;     // bytes from this lane's unit on
             u32x4 v = zero;
-            if (left > 0)
-                v = clear_tail(*reinterpret_cast<const u32x4 *>(g.a + static_cast<int64_t>(m0) * g.lda + at + a_voff[j]), left);
-            *reinterpret_cast<u32x4 *>(smem + (wave + NW * j) * 1024 + lane * 16) = v;
+            if (here > 0)
+                v = clear_tail(*reinterpret_cast<const u32x4 *>(g.a + static_cast<int64_t>(m0) * g.lda + at + a_voff[j]), here);
+            *reinterpret_cast<u32x4 *>(smem + stage + (wave + NW * j) * 1024 + lane * 16) = v;
         }
 #pragma unroll
         for (int j = 0; j < B_LOADS; ++j) {
             u32x4 v = zero;
-            if (left > 0) v = *reinterpret_cast<const u32x4 *>(g.w + static_cast<int64_t>(n0) * g.ldw + at + b_voff[j]);
-            *reinterpret_cast<u32x4 *>(smem + kAStage + (wave + NW * j) * 1024 + lane * 16) = v;
+            if (left > piece_unit(wave + NW * j) * 16)
+                v = *reinterpret_cast<const u32x4 *>(g.w + static_cast<int64_t>(n0) * g.ldw + at + b_voff[j]);
+            *reinterpret_cast<u32x4 *>(smem + stage + kAStage + (wave + NW * j) * 1024 + lane * 16) = v;
         }
         __syncthreads();
-        static_for<kFragOps>([&](auto o_tag) {
-            frag_op(0, 0, Slot0{}, o_tag);
-            frag_op(0, 1, Slot1{}, o_tag);
-        });
-        static_for<NM>([&](auto q_tag) {
-            mfma_at(Slot0{}, q_tag);
-            mfma_at(Slot1{}, q_tag);
+        static_for<CHUNKS>([&](auto c_tag) {
+            constexpr int c = decltype(c_tag)::value;
+            static_for<kFragOps>([&](auto o_tag) { frag_op(c, Slot0{}, o_tag); });
+            static_for<NM>([&](auto q_tag) { mfma_at(Slot0{}, q_tag); });
         });
     }
 
+    // The sums go through LDS, 32 rows of a wavefront's tile at a time, so that a lane has eight neighbouring
+    // outputs of a row: whole 16-byte accesses to c and the residual (an output per lane, 2 bytes each,
+    // took 150 us of a 417 us product of 4096 x 8192 x 8192 with a residual).
+    __syncthreads();
+    constexpr int kCols = 32 * TN, kPad = kCols + 4, kLanesPerRow = kCols / 8, kRowsPerTrip = kWave / kLanesPerRow;
+    constexpr int kTrips = 32 / kRowsPerTrip;
+    static_assert(NW * 32 * kPad * 4 <= 2 * kStage, "room in the stages");
+    int32_t *mine = reinterpret_cast<int32_t *>(smem) + wave * 32 * kPad;
+    const int col = n0 + wn * kCols + lane % kLanesPerRow * 8;
+    float sw[8];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int col = n0 + (wn * TN + j) * 32 + l32;
-        if (col >= g.n) continue;
-        const float sw = g.w_scale[col];
+    for (int e = 0; e < 8; ++e) sw[e] = g.w_scale[min(col + e, g.n - 1)];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i) {
+        T res[kTrips][8];
+        const int row0 = m0 + (wm * TM + i) * 32 + lane / kLanesPerRow;
+        if (g.wide && g.residual && col < g.n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = m0 + (wm * TM + i) * 32 + 8 * (r / 4) + 4 * half + (r % 4);
-                if (row < g.m) store_scaled(g, row, col, acc[i][j][r], g.a_scale[row], sw);
+            for (int q = 0; q < kTrips; ++q) {
+                const int row = min(row0 + q * kRowsPerTrip, g.m - 1);
+#pragma unroll
+                for (size_t u = 0; u < sizeof(T) / 2; ++u)
+                    reinterpret_cast<u32x4 *>(res[q])[u] =
+                        reinterpret_cast<const u32x4 *>(g.residual + row * g.ldr + col)[u];
             }
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine[(8 * (r / 4) + 4 * half + r % 4) * kPad + j * 32 + l32] = acc[i][j][r];
+        // (a wavefront reads back what it wrote itself: its LDS accesses stay in order)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < kTrips; ++q) {
+            const int row = row0 + q * kRowsPerTrip;
+            int32_t sum[8];
+            const int32_t *from = mine + (lane / kLanesPerRow + q * kRowsPerTrip) * kPad + lane % kLanesPerRow * 8;
+            *reinterpret_cast<u32x4 *>(sum) = *reinterpret_cast<const u32x4 *>(from);
+            *reinterpret_cast<u32x4 *>(sum + 4) = *reinterpret_cast<const u32x4 *>(from + 4);
+            if (row >= g.m || col >= g.n) continue;
+            const float sa = g.a_scale[row];
+            if (g.wide) {
+                T out[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float v = static_cast<float>(sum[e]) * sa * sw[e];
+                    if (g.residual) v += to_float(res[q][e]);
+                    out[e] = static_cast<T>(v);
+                }
+#pragma unroll
+                for (size_t u = 0; u < sizeof(T) / 2; ++u)
+                    reinterpret_cast<u32x4 *>(g.c + row * g.ldc + col)[u] = reinterpret_cast<u32x4 *>(out)[u];
+            } else {
+                for (int e = 0; e < 8 && col + e < g.n; ++e) store_scaled(g, row, col + e, sum[e], sa, sw[e]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -308,15 +363,15 @@ int32_t launch_few_rows(hipStream_t st, const Int8Args<T> &g) {
     return launch_status();
 }
 
-template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+template <typename T, int TM, int TN, int WM, int WN>
 int32_t launch_tiles(hipStream_t st, Int8Args<T> g) {
-    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, lds = STAGES * (BM + BN) * 64;
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, lds = 2 * (BM + BN) * 128;
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     g.tiles_m = (g.m + BM - 1) / BM;
     g.tiles_n = (g.n + BN - 1) / BN;
     const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
     if (tiles > (1 << 21)) return RMLK_ERR_TOO_LARGE;
-    auto kern = int8_tiles_kernel<T, TM, TN, WM, WN, STAGES>;
+    auto kern = int8_tiles_kernel<T, TM, TN, WM, WN>;
     static DynamicLdsGrant grant;
     if (const int32_t bad = grant.ensure(kern, lds); bad != RMLK_OK) return bad;
     kern<<<static_cast<uint32_t>((tiles + 7) / 8 * 8), WM * WN * kWave, lds, st>>>(g);
@@ -332,8 +387,8 @@ int32_t launch_int8(hipStream_t st, const Int8Args<T> &g) {
         return launch_few_rows<T, 4, 8>(st, g);
     }
     const int64_t big = static_cast<int64_t>((g.m + 255) / 256) * ((g.n + 255) / 256);
-    if (big >= kNumCU * 3 / 4) return launch_tiles<T, 4, 2, 2, 4, 4>(st, g);
-    return launch_tiles<T, 2, 2, 2, 2, 4>(st, g);
+    if (big >= kNumCU * 3 / 4) return launch_tiles<T, 4, 2, 2, 4>(st, g);
+    return launch_tiles<T, 2, 2, 2, 2>(st, g);
 }
 
 }  // namespace
@@ -378,6 +433,9 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
         g.m = static_cast<int32_t>(m);
         g.n = static_cast<int32_t>(n);
         g.k = static_cast<int32_t>(k);
+        constexpr int64_t unit = 16 / sizeof(T);
+        g.wide = n % 8 == 0 && ldc % unit == 0 && aligned16(c) &&
+                 (!residual || (ldr % unit == 0 && aligned16(residual)));
         return launch_int8(st, g);
     });
 }
