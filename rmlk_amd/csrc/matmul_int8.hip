@@ -2,9 +2,10 @@
 // The integer sums are exact in 32 bits (k < 2^17, |values| <= 128), whatever their order; the
 // epilogue scales them in float and rounds once to the output type.
 //
-// Two kernels. Up to 64 rows the weights are what is read, once: a block takes 16 channels and all the
-// rows, its wavefronts deal K out among themselves and meet in LDS (int8_few_rows_kernel). Beyond, tiles
-// of a and wt go through LDS (int8_tiles_kernel).
+// Three kernels. With few rows the weights are what is read, once: a block takes 16 channels and all the
+// rows, its wavefronts deal K out among themselves and meet in LDS (int8_few_rows_kernel), or, given
+// channels enough, a block streams tiles of channels past rows that it keeps (int8_wide_kernel).
+// Beyond, tiles of a and wt go through LDS (int8_tiles_kernel).
 #include "paged.hpp"
 
 namespace rmlk {
@@ -24,6 +25,8 @@ struct Int8Args {
     int64_t lda, ldw, ldr, ldc;
     int32_t m, n, k;
     int32_t tiles_m, tiles_n;
+    int32_t *sums;       // K split over blocks: the integer sums [splits][m][n rounded up to 8]
+    int32_t k_per_split;
     int32_t wide;        // eight outputs (and residuals) of a row are whole 16-byte units
 };
 
@@ -64,10 +67,10 @@ __global__ __launch_bounds__(WAVES *kWave) void int8_few_rows_kernel(Int8Args<T>
         u32x4 wv[4], av[4][MT];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int at = k0 + j * 64 + lane / 16 * 16;
-            wv[j] = *reinterpret_cast<const u32x4 *>(w + (at < g.k ? at : 0));
+            const int at = k0 + j * 64 + lane / 16 * 16, from = at < g.k ? at : 0;
+            wv[j] = *reinterpret_cast<const u32x4 *>(w + from);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) av[j][t] = *reinterpret_cast<const u32x4 *>(a[t] + (at < g.k ? at : 0));
+            for (int t = 0; t < MT; ++t) av[j][t] = *reinterpret_cast<const u32x4 *>(a[t] + from);
         }
         if (k0 + 256 > g.k) {
 #pragma unroll
@@ -96,16 +99,84 @@ __global__ __launch_bounds__(WAVES *kWave) void int8_few_rows_kernel(Int8Args<T>
     }
 }
 
+// The same for many channels and more than a few rows: a block keeps its share of a in registers (KU units
+// of 64 bytes of K per wavefront) and streams tile after tile of 16 channels past it, the loads of the
+// next tile in flight while one is summed up; the sums meet in two LDS buffers in turn, one barrier per
+// tile. The block's wavefronts read whole rows of weights together. Bound by the memory: 8 rows, 128256
+// channels, K = 2048 take 50 us (5.3 TB/s), the kernel above, which reads a again for every tile, 55 us;
+// with one row 45 and 41 us. Measured and dropped: tiles of 32 and 64 channels (51 and 56 us), runs of
+// neighbouring tiles per block (55 us), a wavefront per tile with a in LDS (51 us).
+constexpr int kWideWaves = 8;
+template <typename T, int MT, int KU>
+__global__ __launch_bounds__(kWideWaves *kWave) void int8_wide_kernel(Int8Args<T> g) {
+    __shared__ int32_t parts[2][kWideWaves][MT][kWave][4];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int tiles = (g.n + 15) / 16;
+    // wavefront w takes the units w, w + 8, ..: a tile's loads of one j cover 512 bytes of every row
+    u32x4 av[KU][MT];
+    int from[KU];
+#pragma unroll
+    for (int j = 0; j < KU; ++j) {
+        const int at = (j * kWideWaves + wave) * 64 + lane / 16 * 16;
+        from[j] = at < g.k ? at : 0;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int8_t *a = g.a + static_cast<int64_t>(min(t * 16 + lane % 16, g.m - 1)) * g.lda;
+            av[j][t] = clear_tail(*reinterpret_cast<const u32x4 *>(a + from[j]), g.k - at);
+        }
+    }
+    auto fetch = [&](u32x4 (&to)[KU], int tile) {
+        const int8_t *w = g.w + static_cast<int64_t>(min(tile * 16 + lane % 16, g.n - 1)) * g.ldw;
+#pragma unroll
+        for (int j = 0; j < KU; ++j) to[j] = *reinterpret_cast<const u32x4 *>(w + from[j]);
+    };
+    u32x4 now[KU], next[KU];
+    int tile = blockIdx.x;
+    fetch(now, tile);
+    auto one_tile = [&](u32x4 (&cur)[KU], u32x4 (&ahead)[KU], int buf) {
+        const int after = tile + gridDim.x;
+        if (after < tiles) fetch(ahead, after);
+        v4i acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, cur[j]),
+                                                               __builtin_bit_cast(v4i, av[j][t]), acc[t], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) *reinterpret_cast<v4i *>(parts[buf][wave][t][lane]) = acc[t];
+        // (a buffer is written again two tiles later, behind the barrier of the tile between)
+        __syncthreads();
+        for (int i = tid; i < MT * 256; i += kWideWaves * kWave) {
+            const int row = i / 16, col = i % 16, n = tile * 16 + col;
+            if (row >= g.m || n >= g.n) continue;
+            int32_t sum = 0;
+#pragma unroll
+            for (int v = 0; v < kWideWaves; ++v) sum += parts[buf][v][row / 16][row % 16 + col / 4 * 16][col % 4];
+            store_scaled(g, row, n, sum, g.a_scale[row], g.w_scale[n]);
+        }
+        tile = after;
+        return after < tiles;
+    };
+    while (true) {
+        if (!one_tile(now, next, 0)) break;
+        if (!one_tile(next, now, 1)) break;
+    }
+}
+
 // Block tile (32 TM WM) x (32 TN WN), WM x WN wavefronts of 32 TM x 32 TN, K steps of 128 bytes: whole
 // cache lines (with steps of 64 bytes every line crossed from the L2 twice).
 // LDS rows are 128 bytes (eight 16-byte units), unpadded - a direct load writes 64 lanes x 16 bytes as one
 // contiguous KiB, eight rows - and unit u of row r lives at position u ^ ((r >> 1) & 7) of its row, so
-// that the sixteen lanes a 128-bit fragment read serves together cover all banks once. Two stages: the
-// one for K step s + 1 is requested in the first quarter of step s into the one read in step s - 1; one
-// barrier per K step, in its last quarter, behind which the first fragments of the next step are read.
-// LDS reads and direct loads are dealt out between the MFMAs. Rows behind m and n are read from the last
+// that the sixteen lanes a 128-bit fragment read serves together cover all banks once. The stage for K
+// step s + STAGES - 1 is requested in the first quarter of step s into the one read in step s - 1 (loads
+// complete in order: vmcnt tells when the next stage is there); one barrier per K step, in its last
+// quarter, behind which the first fragments of the next step are read. LDS reads and direct loads are
+// dealt out between the MFMAs. Rows behind m and n are read from the last
 // row and not stored.
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, CHUNKS = 4;
     constexpr int kAStage = BM * BK, kStage = (BM + BN) * BK;
@@ -123,7 +194,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     const int in_group = t - group * GM * g.tiles_n;
     const int tile_m = first_m + in_group % gm, tile_n = in_group / gm;
     const int m0 = tile_m * BM, n0 = tile_n * BN;
-    const int n_steps = g.k / BK;
+    const int k_begin = blockIdx.y * g.k_per_split, k_here = min(g.k - k_begin, g.k_per_split);
+    const int n_steps = k_here / BK;
 
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int wm = wave / WN, wn = wave % WN;
@@ -143,8 +215,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         const int q = wave + NW * j;
         b_voff[j] = static_cast<uint32_t>(min(piece_row(q), g.n - 1 - n0) * g.ldw + piece_unit(q) * 16);
     }
-    const int8_t *a_ptr = g.a + static_cast<int64_t>(m0) * g.lda;
-    const int8_t *b_ptr = g.w + static_cast<int64_t>(n0) * g.ldw;
+    const int8_t *a_ptr = g.a + static_cast<int64_t>(m0) * g.lda + k_begin;
+    const int8_t *b_ptr = g.w + static_cast<int64_t>(n0) * g.ldw + k_begin;
     const uint32_t lds0 =
         __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + wave * 1024u);
 
@@ -167,8 +239,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         b_ptr += BK;
     };
 
-    // LDS addresses of the fragments of every chunk, moved to the other stage at the end of a step
-    static_assert((kStage & (kStage - 1)) == 0, "stages are told apart by one address bit");
+    // LDS addresses of the fragments of every chunk, moved to the next stage at the end of a step
     uint32_t a_addr[CHUNKS], b_addr[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -183,11 +254,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         if constexpr (o < TN) bf[s][o] = *reinterpret_cast<const u32x4 *>(smem + b_addr[c] + o * 32 * BK);
         else af[s][o - TN] = *reinterpret_cast<const u32x4 *>(smem + a_addr[c] + (o - TN) * 32 * BK);
     };
-    auto other_stage = [&]() {
+    int stage = 0;
+    auto next_stage = [&]() {
+        const uint32_t move = stage + 1 == STAGES ? -(STAGES - 1) * kStage : kStage;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            a_addr[c] ^= kStage;
-            b_addr[c] ^= kStage;
+            a_addr[c] += move;
+            b_addr[c] += move;
         }
     };
 
@@ -208,8 +282,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     using Slot0 = std::integral_constant<int, 0>;
     using Slot1 = std::integral_constant<int, 1>;
     constexpr int kBarrierAt = NM / 4;
-    auto k_step = [&](int fill, auto more_tag) {
-        constexpr bool MORE = decltype(more_tag)::value;
+    auto k_step = [&](int fill, auto load_tag, auto more_tag) {
+        constexpr bool LOAD = decltype(load_tag)::value, MORE = decltype(more_tag)::value;
         static_for<CHUNKS - 1>([&](auto c_tag) {
             constexpr int c = decltype(c_tag)::value;
             using Now = std::integral_constant<int, c % 2>;
@@ -221,7 +295,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                     constexpr int o = decltype(o_tag)::value;
                     if constexpr (o * NM / kFragOps == q) frag_op(c + 1, Next{}, o_tag);
                 });
-                if constexpr (MORE && c == 0)
+                if constexpr (LOAD && c == 0)
                     static_for<kLoads>([&](auto o_tag) {
                         constexpr int o = decltype(o_tag)::value;
                         if constexpr (o * NM / kLoads == q) load_op(fill, o_tag);
@@ -229,7 +303,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
-        if constexpr (MORE) {
+        if constexpr (LOAD) {
             a_ptr += BK;
             b_ptr += BK;
         }
@@ -240,14 +314,18 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
             if constexpr (MORE && q == kBarrierAt) {
                 // this wavefront has read all of this stage and its part of the next one has landed;
                 // then the block meets
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                if constexpr (LOAD)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 asm volatile("s_barrier" ::: "memory");
-                other_stage();
+                next_stage();
             }
             if constexpr (MORE) {
                 static_for<kFragOps>([&](auto o_tag) {
                     constexpr int o = decltype(o_tag)::value;
-                    if constexpr (kBarrierAt + 1 + (kFragOps <= room ? o : o * room / kFragOps) == q)
+                    constexpr int place = kBarrierAt + 1 + (kFragOps <= room ? o : o * room / kFragOps);
+                    if constexpr ((place < NM ? place : NM - 1) == q)
                         frag_op(0, Slot0{}, o_tag);
                 });
             }
@@ -256,23 +334,26 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     };
 
     if (n_steps > 0) {
-        load_stage(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const int pre = n_steps < STAGES - 1 ? n_steps : STAGES - 1;
+        for (int i = 0; i < pre; ++i) load_stage(i);
+        if (pre == STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
         static_for<kFragOps>([&](auto o_tag) { frag_op(0, Slot0{}, o_tag); });
-        int fill = 1;
-        for (int step = 1; step < n_steps; ++step) {
-            k_step(fill, std::true_type{});
-            fill ^= 1;
+        int fill = STAGES - 1, step = 0;
+        for (; step + STAGES - 1 < n_steps; ++step) {
+            k_step(fill, std::true_type{}, std::true_type{});
+            fill = fill + 1 == STAGES ? 0 : fill + 1;
         }
-        k_step(fill, std::false_type{});
+        if constexpr (STAGES > 2)
+            for (; step + 1 < n_steps; ++step) k_step(0, std::false_type{}, std::true_type{});
+        k_step(0, std::false_type{}, std::false_type{});
     }
-    if (g.k % BK != 0) {
+    if (k_here % BK != 0) {
         // the rest of K, through registers: what lies behind k is zero in a
         __syncthreads();
-        const int left = g.k - n_steps * BK;
-        const int stage = n_steps > 1 && n_steps % 2 == 0 ? kStage : 0;      // where the fragment addresses point
-        const int64_t at = static_cast<int64_t>(n_steps) * BK;
+        const int left = k_here - n_steps * BK;
+        const int64_t at = k_begin + static_cast<int64_t>(n_steps) * BK;
         const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < A_LOADS; ++j) {
@@ -280,14 +361,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
             u32x4 v = zero;
             if (here > 0)
                 v = clear_tail(*reinterpret_cast<const u32x4 *>(g.a + static_cast<int64_t>(m0) * g.lda + at + a_voff[j]), here);
-            *reinterpret_cast<u32x4 *>(smem + stage + (wave + NW * j) * 1024 + lane * 16) = v;
+            *reinterpret_cast<u32x4 *>(smem + stage * kStage + (wave + NW * j) * 1024 + lane * 16) = v;
         }
 #pragma unroll
         for (int j = 0; j < B_LOADS; ++j) {
             u32x4 v = zero;
             if (left > piece_unit(wave + NW * j) * 16)
                 v = *reinterpret_cast<const u32x4 *>(g.w + static_cast<int64_t>(n0) * g.ldw + at + b_voff[j]);
-            *reinterpret_cast<u32x4 *>(smem + stage + kAStage + (wave + NW * j) * 1024 + lane * 16) = v;
+            *reinterpret_cast<u32x4 *>(smem + stage * kStage + kAStage + (wave + NW * j) * 1024 + lane * 16) = v;
         }
         __syncthreads();
         static_for<CHUNKS>([&](auto c_tag) {
@@ -303,7 +384,6 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     __syncthreads();
     constexpr int kCols = 32 * TN, kPad = kCols + 4, kLanesPerRow = kCols / 8, kRowsPerTrip = kWave / kLanesPerRow;
     constexpr int kTrips = 32 / kRowsPerTrip;
-    static_assert(NW * 32 * kPad * 4 <= 2 * kStage, "room in the stages");
     int32_t *mine = reinterpret_cast<int32_t *>(smem) + wave * 32 * kPad;
     const int col = n0 + wn * kCols + lane % kLanesPerRow * 8;
     float sw[8];
@@ -313,7 +393,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     for (int i = 0; i < TM; ++i) {
         T res[kTrips][8];
         const int row0 = m0 + (wm * TM + i) * 32 + lane / kLanesPerRow;
-        if (g.wide && g.residual && col < g.n) {
+        if (g.wide && g.residual && !g.sums && col < g.n) {
 #pragma unroll
             for (int q = 0; q < kTrips; ++q) {
                 const int row = min(row0 + q * kRowsPerTrip, g.m - 1);
@@ -337,6 +417,12 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
             *reinterpret_cast<u32x4 *>(sum) = *reinterpret_cast<const u32x4 *>(from);
             *reinterpret_cast<u32x4 *>(sum + 4) = *reinterpret_cast<const u32x4 *>(from + 4);
             if (row >= g.m || col >= g.n) continue;
+            if (g.sums) {
+                int32_t *to = g.sums + (static_cast<int64_t>(blockIdx.y) * g.m + row) * ((g.n + 7) & ~7) + col;
+                *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<u32x4 *>(sum);
+                *reinterpret_cast<u32x4 *>(to + 4) = *reinterpret_cast<u32x4 *>(sum + 4);
+                continue;
+            }
             const float sa = g.a_scale[row];
             if (g.wide) {
                 T out[8];
@@ -357,38 +443,110 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     }
 }
 
+// The splits of K joined: eight outputs of a row per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_join_kernel(Int8Args<T> g, int32_t splits) {
+    const int units = (g.n + 7) / 8;
+    const int64_t slab = static_cast<int64_t>(g.m) * units * 8;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<int64_t>(g.m) * units;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int row = static_cast<int>(i / units), col = static_cast<int>(i % units) * 8;
+        v4i lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        for (int s = 0; s < splits; ++s) {
+            const v4i *from = reinterpret_cast<const v4i *>(g.sums + s * slab + i * 8);
+            lo += from[0];
+            hi += from[1];
+        }
+        const float sa = g.a_scale[row];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < g.n) store_scaled(g, row, col + e, e < 4 ? lo[e] : hi[e - 4], sa, g.w_scale[col + e]);
+    }
+}
+
 template <typename T, int MT, int WAVES>
 int32_t launch_few_rows(hipStream_t st, const Int8Args<T> &g) {
     int8_few_rows_kernel<T, MT, WAVES><<<static_cast<uint32_t>((g.n + 15) / 16), WAVES * kWave, 0, st>>>(g);
     return launch_status();
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
-int32_t launch_tiles(hipStream_t st, Int8Args<T> g) {
-    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, lds = 2 * (BM + BN) * 128;
+template <typename T, int MT, int KU>
+int32_t launch_wide(hipStream_t st, const Int8Args<T> &g) {
+    const int64_t tiles = (static_cast<int64_t>(g.n) + 15) / 16, resident = 2 * kNumCU;
+    int8_wide_kernel<T, MT, KU>
+        <<<static_cast<uint32_t>(tiles < resident ? tiles : resident), kWideWaves * kWave, 0, st>>>(g);
+    return launch_status();
+}
+
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+int32_t launch_tiles(hipStream_t st, Int8Args<T> g, int32_t splits) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, stages = STAGES * (BM + BN) * 128;
+    constexpr int sums = WM * WN * 32 * (32 * TN + 4) * 4, lds = stages > sums ? stages : sums;
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     g.tiles_m = (g.m + BM - 1) / BM;
     g.tiles_n = (g.n + BN - 1) / BN;
     const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
     if (tiles > (1 << 21)) return RMLK_ERR_TOO_LARGE;
-    auto kern = int8_tiles_kernel<T, TM, TN, WM, WN>;
+    auto kern = int8_tiles_kernel<T, TM, TN, WM, WN, STAGES>;
     static DynamicLdsGrant grant;
     if (const int32_t bad = grant.ensure(kern, lds); bad != RMLK_OK) return bad;
-    kern<<<static_cast<uint32_t>((tiles + 7) / 8 * 8), WM * WN * kWave, lds, st>>>(g);
+    kern<<<dim3(static_cast<uint32_t>((tiles + 7) / 8 * 8), static_cast<uint32_t>(splits)), WM * WN * kWave, lds, st>>>(g);
     return launch_status();
 }
 
-template <typename T>
-int32_t launch_int8(hipStream_t st, const Int8Args<T> &g) {
-    if (g.m <= 64) {
-        const bool wide = static_cast<int64_t>(g.n) >= 16 * 2 * kNumCU;   // blocks enough for every unit
-        if (g.m <= 16) return wide ? launch_few_rows<T, 1, 8>(st, g) : launch_few_rows<T, 1, 16>(st, g);
-        if (g.m <= 32) return launch_few_rows<T, 2, 8>(st, g);
-        return launch_few_rows<T, 4, 8>(st, g);
+// Which kernel a size takes, and the splits of K.
+enum Route { kFewRows, kWide, kTile64, kTile64x128, kTile128, kTile256 };
+struct Plan {
+    Route route;
+    int32_t splits, k_per_split;
+};
+Plan plan_for(int64_t m, int64_t n, int64_t k) {
+    auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
+    Plan p{kTile64, 1, static_cast<int32_t>(k)};
+    if (m > 4 && m <= 32 && n >= 64 * kNumCU && k <= 4096) {
+        p.route = kWide;
+    } else if (m <= 16 || (m <= 32 && n * k <= (1 << 23))) {
+        p.route = kFewRows;
+    } else if (m > 128 && tiles(256, 256) >= kNumCU * 3 / 4) {
+        p.route = kTile256;
+    } else if (m > 64 && tiles(128, 128) >= kNumCU * 11 / 16) {
+        p.route = kTile128;
+    } else if (tiles(64, 128) >= kNumCU) {
+        p.route = kTile64x128;
+    } else {
+        // fewer tiles than compute units: a long K is split, at least 1024 bytes of it per block (the join is a
+        // launch of 3 us; 128 x 2048 x 2048 takes 7 us in one piece, 11 us in four)
+        int64_t s = kNumCU / tiles(64, 64);
+        s = s < k / 1024 ? s : k / 1024;
+        s = s < 8 ? s : 8;
+        if (s > 1 && k >= 4096) {
+            const int64_t per = ((k + s - 1) / s + 127) / 128 * 128;
+            p.k_per_split = static_cast<int32_t>(per);
+            p.splits = static_cast<int32_t>((k + per - 1) / per);
+        }
     }
-    const int64_t big = static_cast<int64_t>((g.m + 255) / 256) * ((g.n + 255) / 256);
-    if (big >= kNumCU * 3 / 4) return launch_tiles<T, 4, 2, 2, 4>(st, g);
-    return launch_tiles<T, 2, 2, 2, 2>(st, g);
+    return p;
+}
+
+template <typename T>
+int32_t launch_int8(hipStream_t st, Int8Args<T> g, const Plan &p, void *workspace) {
+    g.k_per_split = p.k_per_split;
+    g.sums = p.splits > 1 ? static_cast<int32_t *>(workspace) : nullptr;
+    switch (p.route) {
+        case kFewRows:
+            if (g.m > 16) return launch_few_rows<T, 2, 8>(st, g);
+            return g.n >= 16 * 2 * kNumCU ? launch_few_rows<T, 1, 8>(st, g) : launch_few_rows<T, 1, 16>(st, g);
+        case kWide:
+            if (g.m > 16) return g.k <= 2048 ? launch_wide<T, 2, 4>(st, g) : launch_wide<T, 2, 8>(st, g);
+            return g.k <= 2048 ? launch_wide<T, 1, 4>(st, g) : launch_wide<T, 1, 8>(st, g);
+        case kTile256: return launch_tiles<T, 4, 2, 2, 4, 2>(st, g, 1);
+        case kTile128: return launch_tiles<T, 1, 2, 4, 2, 4>(st, g, 1);
+        case kTile64x128: return launch_tiles<T, 1, 2, 2, 2, 3>(st, g, 1);
+        case kTile64: break;
+    }
+    if (const int32_t bad = launch_tiles<T, 1, 1, 2, 2, 4>(st, g, p.splits); bad != RMLK_OK || p.splits == 1) return bad;
+    int8_join_kernel<T><<<grid_for(static_cast<int64_t>(g.m) * ((g.n + 7) / 8), 256), 256, 0, st>>>(g, p.splits);
+    return launch_status();
 }
 
 }  // namespace
@@ -398,7 +556,11 @@ using namespace rmlk;
 
 extern "C" {
 
-size_t rmlk_hip_matmul_int8_workspace_size(int64_t, int64_t, int64_t) { return 0; }
+size_t rmlk_hip_matmul_int8_workspace_size(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    const Plan p = plan_for(m, n, k);
+    return p.splits > 1 ? static_cast<size_t>(p.splits) * m * ((n + 7) / 8 * 8) * sizeof(int32_t) : 0;
+}
 
 int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int64_t n, int64_t k, const void *a,
                              int64_t lda, const float *a_scale, const void *wt, int64_t ldw, const float *w_scale,
@@ -415,6 +577,7 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
     const size_t need = rmlk_hip_matmul_int8_workspace_size(m, n, k);
     if (need > 0) {
         if (!workspace) return RMLK_ERR_NULL_POINTER;
+        if (!aligned16(workspace)) return RMLK_ERR_UNSUPPORTED;
         if (workspace_bytes < need) return RMLK_ERR_WORKSPACE;
     }
     return with_activation(dtype, [&](auto tag) {
@@ -436,7 +599,7 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
         constexpr int64_t unit = 16 / sizeof(T);
         g.wide = n % 8 == 0 && ldc % unit == 0 && aligned16(c) &&
                  (!residual || (ldr % unit == 0 && aligned16(residual)));
-        return launch_int8(st, g);
+        return launch_int8(st, g, plan_for(m, n, k), workspace);
     });
 }
 

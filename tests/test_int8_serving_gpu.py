@@ -184,7 +184,9 @@ def _product_case(device, kind, m, n, k, residual, seed, lda=None, values=127):
     (1, 16, 32), (1, 2048, 2048), (1, 33, 100), (2, 128, 64), (3, 1000, 4096), (7, 65, 8192), (8, 130, 2048),
     (16, 512, 512), (17, 515, 1040), (31, 64, 16), (33, 257, 272), (64, 256, 1024), (65, 129, 640), (100, 640, 320),
     (128, 256, 256), (129, 257, 129), (200, 2048, 2048), (256, 1024, 5000), (300, 770, 1), (509, 1024, 2048),
-    (1, 1, 1), (1, 5000, 31), (12, 4096, 48), (48, 48, 4800)])
+    (1, 1, 1), (1, 5000, 31), (12, 4096, 48), (48, 48, 4800), (6, 16400, 100), (8, 16384, 2064), (20, 17000, 530),
+    (32, 16387, 4096), (4, 20000, 64), (64, 100, 8200), (40, 70, 131071), (300, 130, 9000), (513, 33000, 64),
+    (256, 12300, 150), (70, 40000, 96)])
 def test_matmul_int8_sizes(device, m, n, k):
     _product_case(device, "f32", m, n, k, None, m * 31 + n * 7 + k)
 
