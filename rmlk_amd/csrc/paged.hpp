@@ -109,64 +109,62 @@ inline int32_t paged_pointers(const rmlk_paged_cache *cache, const rmlk_paged_ba
     return RMLK_OK;
 }
 
-// Rows, new tokens and length of sequence s; false for one whose numbers contradict the call's bounds.
+// Rows, new tokens and length of a sequence, and whether they keep to the call's bounds.
 struct Sequence {
     int32_t row;       // its first row
     int32_t fresh;     // its rows
     int32_t length;    // tokens it holds, these included
 };
-__device__ __forceinline__ bool sequence_at(const PagedArgs &g, int s, Sequence &q) {
-    const int32_t lo = g.first[s], hi = g.first[s + 1];
-    q.row = lo;
-    q.fresh = hi - lo;
-    q.length = g.length[s];
-    return lo >= 0 && hi >= lo && hi <= g.rows && hi - lo <= g.max_new && q.length >= 0 && q.length <= g.max_length;
+// (`first` ascends within the rows: locate has said so)
+__device__ __forceinline__ bool in_bounds(const PagedArgs &g, const Sequence &q) {
+    return q.fresh <= g.max_new && q.length >= 0 && q.length <= g.max_length;
 }
 
-// first[0 .. seqs] ascends within 0 .. rows (checked by every wavefront for itself: the array is a few
-// cache lines).
-__device__ __forceinline__ bool starts_ascend(const PagedArgs &g) {
+// One trip over `first` and `length` by every wavefront for itself (a few cache lines): false when `first`
+// does not ascend within 0 .. rows; otherwise the last sequence s with begins(first[s], s), which has to hold
+// for a run of sequences from 0 on, and its numbers (s = -1: none). The work of a ragged call is numbered
+// so that sequence s has the numbers from first[s] / unit + extra * s on, floor(its rows / unit) + extra of
+// them at least: a grid of rows / unit + extra * seqs blocks covers every sequence without a rectangle over
+// the longest one.
+template <typename F>
+__device__ __forceinline__ bool locate(const PagedArgs &g, F &&begins, int &s, Sequence &q) {
+    s = -1;
     bool good = true;
-    for (int i = static_cast<int>(threadIdx.x % kWave); i < g.seqs; i += kWave) {
-        const int32_t lo = g.first[i], hi = g.first[i + 1];
-        good = good && lo >= 0 && lo <= hi && hi <= g.rows;
+    for (int base = 0; base < g.seqs; base += kWave) {
+        const int i = base + static_cast<int>(threadIdx.x % kWave);
+        int32_t lo = 0, hi = 0, length = 0;
+        bool before = false;
+        if (i < g.seqs) {
+            lo = g.first[i];
+            hi = g.first[i + 1];
+            length = g.length[i];
+            good = good && lo >= 0 && lo <= hi && hi <= g.rows;
+            before = begins(lo, i);
+        }
+        const int n = __popcll(__ballot(before));
+        if (n > 0) {
+            s = base + n - 1;
+            q.row = __builtin_amdgcn_readlane(lo, n - 1);
+            q.fresh = __builtin_amdgcn_readlane(hi, n - 1) - q.row;
+            q.length = __builtin_amdgcn_readlane(length, n - 1);
+        }
     }
     return __all(good);
 }
 
-// The work of a ragged call in pieces of `unit` (a power of two or not) rows: sequence s has the numbers
-// from first[s] / unit + extra * s on, floor(rows / unit) + extra of them at least, so that a grid of
-// rows / unit + extra * seqs blocks covers every sequence without a rectangle over the longest one.
-// A wavefront counts the sequences that begin at or before `piece`; -1 with no sequence.
-__device__ __forceinline__ int sequence_of(const PagedArgs &g, int piece, int unit, int extra) {
-    int s = -1;
-    for (int base = 0; base < g.seqs; base += kWave) {
-        const int i = base + static_cast<int>(threadIdx.x % kWave);
-        s += __popcll(__ballot(i < g.seqs && g.first[i] / unit + extra * i <= piece));
-    }
-    return s;
-}
-
-// The same over rep rows of a matrix per row of the call: tile number `piece` of `unit` matrix rows.
-__device__ __forceinline__ int sequence_of_rows(const PagedArgs &g, int piece, int rep, int unit) {
-    int s = -1;
-    for (int base = 0; base < g.seqs; base += kWave) {
-        const int i = base + static_cast<int>(threadIdx.x % kWave);
-        s += __popcll(__ballot(i < g.seqs && g.first[i] * rep / unit + i <= piece));
-    }
-    return s;
-}
-
-// The last sequence that starts at or before a row (of those that share a start: the last, which is
-// the one that has rows).
-__device__ __forceinline__ int sequence_of_row(const PagedArgs &g, int64_t row) {
+// The sequence of a row by bisection, for work whose lanes differ in it (of sequences that share a start: the
+// last, which is the one that has rows).
+__device__ __forceinline__ bool sequence_of_row(const PagedArgs &g, int64_t row, Sequence &q) {
     int lo = 0, hi = g.seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (g.first[mid] <= row) lo = mid;
         else hi = mid;
     }
-    return lo;
+    q.row = g.first[lo];
+    q.fresh = g.first[lo + 1] - q.row;
+    q.length = g.length[lo];
+    return in_bounds(g, q) && row >= q.row && row < q.row + q.fresh;
 }
 
 __device__ __forceinline__ void raise_error(const PagedArgs &g) {

@@ -6,13 +6,15 @@
 // this and the exponent it has; when it grows, the integers held already are shifted right with
 // rounding to nearest even. Rotation and quantisation are evaluated in double (two exact products and
 // one sum): a value next to the border between two integers falls the right way.
+#include <cmath>
+
 #include "paged.hpp"
 
 namespace rmlk {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kLowestExponent = -126;
+constexpr int kHeads = 2;      // heads of q that a thread rotates with one row of the tables
 
 template <typename T>
 struct AppendArgs {
@@ -24,22 +26,8 @@ struct AppendArgs {
     int64_t positions;
     int32_t heads;
     int32_t pieces;      // upper bound of (sequence, page) pairs: the first blocks of the grid, per KV head
-    int64_t q_units;     // rows * heads * D / 16 units of q
+    int64_t q_units;     // units of q: D / 16 per row and kHeads heads
 };
-
-// The pages that sequence s writes to, at most fresh / page_size + 2, are numbered from
-// first[s] / page_size + 2 s: no two sequences share a number, and the grid need not be a rectangle
-// over the longest sequence.
-
-__device__ __forceinline__ double block_max(double v, double *lds) {
-    v = wave_max(v);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    double r = lds[0];
-    for (int i = 1; i < kThreads / kWave; ++i) r = lds[i] > r ? lds[i] : r;
-    __syncthreads();
-    return r;
-}
 
 __device__ __forceinline__ int exponent_for(double a) {
     if (a == 0.0) return kLowestExponent;
@@ -49,58 +37,116 @@ __device__ __forceinline__ int exponent_for(double a) {
     return max(kLowestExponent, min(127, e));
 }
 
-__device__ __forceinline__ int8_t to_step(double x, int e) {
-    const int n = static_cast<int>(rint(ldexp(x, -e)));
-    return static_cast<int8_t>(min(127, max(-127, n)));
+// 2^e as a double, |e| < 1000
+__device__ __forceinline__ double power(int e) {
+    return __longlong_as_double(static_cast<long long>(e + 1023) << 52);
+}
+__device__ __forceinline__ uint32_t to_byte(double x, double inverse_step) {
+    const int n = static_cast<int>(rint(x * inverse_step));
+    return static_cast<uint32_t>(min(127, max(-127, n))) & 255u;
+}
+// (a float times a power of two is exact, or so small that it rounds to zero)
+__device__ __forceinline__ uint32_t to_byte(float x, float inverse_step) {
+    const int n = static_cast<int>(rintf(x * inverse_step));
+    return static_cast<uint32_t>(min(127, max(-127, n))) & 255u;
+}
+__device__ __forceinline__ uint64_t to_bytes(const double (&x)[8], double inverse_step) {
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lo |= to_byte(x[i], inverse_step) << (8 * i);
+        hi |= to_byte(x[4 + i], inverse_step) << (8 * i);
+    }
+    return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-template <typename T, int D>
-__device__ __forceinline__ double rotated(const AppendArgs<T> &g, const T *row, int64_t pos, int d) {
-    const double x = to_float(row[d]);
-    if (!g.cos) return x;
-    const double other = d < D / 2 ? -to_float(row[d + D / 2]) : to_float(row[d - D / 2]);
-    return x * static_cast<double>(g.cos[pos * D + d]) + other * static_cast<double>(g.sin[pos * D + d]);
+// cos and sin of eight dims d .. of the first half of a row and of the eight that rotate with them.
+struct Turn {
+    float c0[8], s0[8], c1[8], s1[8];
+};
+template <int D>
+__device__ __forceinline__ void load_turn(Turn &t, const float *cos, const float *sin, int64_t pos, int d) {
+    load_row(cos + pos * D + d, t.c0);
+    load_row(sin + pos * D + d, t.s0);
+    load_row(cos + pos * D + d + D / 2, t.c1);
+    load_row(sin + pos * D + d + D / 2, t.s1);
+}
+__device__ __forceinline__ void rotate_eight(const float (&a)[8], const float (&b)[8], const Turn &t, bool turn,
+                                             double (&lo)[8], double (&hi)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double x = a[i], y = b[i];
+        lo[i] = turn ? x * t.c0[i] + -y * t.s0[i] : x;
+        hi[i] = turn ? y * t.c1[i] + x * t.s1[i] : y;
+    }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs<T> g) {
-    __shared__ double lds[kThreads / kWave];
-    const int tid = threadIdx.x;
+template <typename T>
+__device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
+#pragma unroll
+    for (size_t u = 0; u < sizeof(T) / 2; ++u) reinterpret_cast<u32x4 *>(to)[u] = reinterpret_cast<const u32x4 *>(v)[u];
+}
+
+// Blocks 0 .. pieces * kv_heads - 1: a block takes one page of one sequence and KV head, K and V. Its threads
+// load all new values of it at once (PK units of 8 + 8 rotating dims of K, 2 PK units of 8 dims of V each),
+// agree on the two largest magnitudes and write: one trip over the values. V is turned in LDS when more
+// than a few tokens come, so that the runs of new slots of a dim go out as whole words. The other blocks
+// rotate q.
+template <typename T, int D, int THREADS, int PK>
+__global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(AppendArgs<T> g) {
+    constexpr int kUnitsK = D / 16, kUnitsV = D / 8;              // units of a token
+    constexpr int kTokensK = THREADS / kUnitsK, kTokensV = THREADS / kUnitsV;   // tokens of one trip
+    constexpr int kMostTokens = PK * kTokensK < 128 ? PK * kTokensK : 128, kPad = kMostTokens + 4;
+    __shared__ double lds[2][THREADS / kWave];
+    __shared__ __align__(16) uint8_t turned[D][kPad];
+    const int tid = threadIdx.x, lane = tid % kWave;
     const int kv_blocks = g.pieces * g.c.kv_heads;
-    if (!starts_ascend(g.c)) {
+    const int piece = blockIdx.x / g.c.kv_heads, head = blockIdx.x % g.c.kv_heads;
+    int s;
+    Sequence q;
+    if (!locate(g.c, [&](int32_t first, int i) { return (first >> g.c.page_shift) + 2 * i <= piece; }, s, q)) {
         if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
         return;
     }
     if (static_cast<int>(blockIdx.x) >= kv_blocks) {
-        // queries: one element per thread and trip
-        const int64_t total = g.c.rows * g.heads * D;
-        for (int64_t i = (static_cast<int64_t>(blockIdx.x) - kv_blocks) * kThreads + tid; i < total;
-             i += static_cast<int64_t>(gridDim.x - kv_blocks) * kThreads) {
-            const int d = static_cast<int>(i % (D / 2));
-            if (i % D >= D / 2) continue;
-            const int64_t rh = i / D;
-            const int64_t row = rh / g.heads;
-            const int h = static_cast<int>(rh % g.heads);
-            Sequence q;
-            if (!sequence_at(g.c, sequence_of_row(g.c, row), q) || q.length < q.fresh || row < q.row ||
-                row >= q.row + q.fresh)
-                continue;
+        const int64_t first_unit = (static_cast<int64_t>(blockIdx.x) - kv_blocks) * THREADS;
+        // a unit: eight + eight dims of kHeads heads of a row, which share their row of the tables
+        const int groups = (g.heads + kHeads - 1) / kHeads;
+        for (int64_t u = first_unit + tid; u < g.q_units; u += static_cast<int64_t>(gridDim.x - kv_blocks) * THREADS) {
+            const int64_t rg = u / kUnitsK;
+            const int d = static_cast<int>(u % kUnitsK) * 8;
+            const int row = static_cast<int>(rg / groups), h0 = static_cast<int>(rg % groups) * kHeads;
+            if (!sequence_of_row(g.c, row, q) || q.length < q.fresh) continue;
             const int64_t pos = q.length - q.fresh + (row - q.row);
             if (g.cos && pos >= g.positions) continue;
-            const T *src = g.q + row * g.q_stride + static_cast<int64_t>(h) * D;
-            const double a = rotated<T, D>(g, src, pos, d), b = rotated<T, D>(g, src, pos, d + D / 2);
-            T *dst = g.q_out + (row * g.heads + h) * D;
-            dst[d] = static_cast<T>(a);
-            dst[d + D / 2] = static_cast<T>(b);
+            const T *from = g.q + row * g.q_stride + d;
+            T *to = g.q_out + static_cast<int64_t>(row) * g.heads * D + d;
+            float x[kHeads][2][8];
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i)
+                if (h0 + i < g.heads) {
+                    load_row(from + (h0 + i) * D, x[i][0]);
+                    load_row(from + (h0 + i) * D + D / 2, x[i][1]);
+                }
+            Turn turn;
+            if (g.cos) load_turn<D>(turn, g.cos, g.sin, pos, d);
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i)
+                if (h0 + i < g.heads) {
+                    double lo[8], hi[8];
+                    rotate_eight(x[i][0], x[i][1], turn, g.cos != nullptr, lo, hi);
+                    store_eight(to + (h0 + i) * D, lo);
+                    store_eight(to + (h0 + i) * D + D / 2, hi);
+                }
         }
         return;
     }
-    const int piece = blockIdx.x / g.c.kv_heads, head = blockIdx.x % g.c.kv_heads;
-    const int s = sequence_of(g.c, piece, 1 << g.c.page_shift, 2);
     if (s < 0) return;
-    const int index = piece - ((g.c.first[s] >> g.c.page_shift) + 2 * s);   // of the pages it writes to
-    Sequence q;
-    if (!sequence_at(g.c, s, q) || q.length < q.fresh) {
+    const int index = piece - ((q.row >> g.c.page_shift) + 2 * s);   // of the pages it writes to
+    if (!in_bounds(g.c, q) || q.length < q.fresh) {
         if (index == 0 && head == 0 && tid == 0) raise_error(g.c);
         return;
     }
@@ -108,9 +154,9 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs<T> g)
     const int begin_pos = q.length - q.fresh;
     const int64_t page_at = static_cast<int64_t>(begin_pos >> g.c.page_shift) + index;   // in the table
     const int64_t page_pos = page_at << g.c.page_shift;
-    if (q.fresh == 0 || page_pos >= q.length) return;
+    if (index < 0 || q.fresh == 0 || page_pos >= q.length) return;
     const int slot0 = page_pos < begin_pos ? static_cast<int>(begin_pos - page_pos) : 0;
-    int slot1 = min(static_cast<int64_t>(size), q.length - page_pos);
+    int slot1 = static_cast<int>(min(static_cast<int64_t>(size), q.length - page_pos));
     const int32_t page = g.c.table[s * g.c.table_stride + page_at];
     if (page < 0 || page >= g.c.pages) {
         if (tid == 0) raise_error(g.c);
@@ -122,48 +168,163 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs<T> g)
         if (slot1 == slot0) return;
     }
     const int tokens = slot1 - slot0;
-    const int64_t row0 = q.row + (page_pos + slot0 - begin_pos);
+    const int64_t row0 = q.row + (page_pos + slot0 - begin_pos), pos0 = page_pos + slot0;
     const int64_t block = static_cast<int64_t>(page) * g.c.kv_heads + head;
-    for (int which = 0; which < 2; ++which) {
-        const T *src = which ? g.v + row0 * g.v_stride : g.k + row0 * g.k_stride;
-        const int64_t stride = which ? g.v_stride : g.k_stride;
-        src += static_cast<int64_t>(head) * D;
-        int8_t *dst = (which ? g.c.v : g.c.k) + block * size * D;
-        float *scale = (which ? g.c.v_scale : g.c.k_scale) + block;
-        auto value = [&](int t, int d) {
-            const T *row = src + t * stride;
-            return which ? static_cast<double>(to_float(row[d])) : rotated<T, D>(g, row, page_pos + slot0 + t, d);
-        };
-        auto at = [&](int slot, int d) { return which ? d * size + slot : slot * D + d; };
-        double top = 0.0;
-        bool finite = true;
-        for (int i = tid; i < tokens * D; i += kThreads) {
-            const double x = value(i / D, i % D);
-            finite = finite && fabs(x) <= 1.7976931348623157e308;
-            top = fabs(x) > top ? fabs(x) : top;
+    int8_t *k_block = g.c.k + block * size * D, *v_block = g.c.v + block * size * D;
+    const float k_held = g.c.k_scale[block], v_held = g.c.v_scale[block];
+
+    double k_lo[PK][8], k_hi[PK][8];
+    float v[2 * PK][8];
+    const int unit_k = tid % kUnitsK * 8, unit_v = tid % kUnitsV * 8;
+#pragma unroll
+    for (int i = 0; i < 2 * PK; ++i) {
+        const int t = i * kTokensV + tid / kUnitsV;
+        if (t < tokens) load_row(g.v + (row0 + t) * g.v_stride + static_cast<int64_t>(head) * D + unit_v, v[i]);
+    }
+    double k_top = 0.0, odd = 0.0;
+    uint32_t v_bits = 0;
+#pragma unroll
+    for (int i = 0; i < PK; ++i) {
+        const int t = i * kTokensK + tid / kUnitsK;
+        if (t < tokens) {
+            const T *from = g.k + (row0 + t) * g.k_stride + static_cast<int64_t>(head) * D + unit_k;
+            float x[2][8];
+            load_row(from, x[0]);
+            load_row(from + D / 2, x[1]);
+            Turn turn;
+            if (g.cos) load_turn<D>(turn, g.cos, g.sin, pos0 + t, unit_k);
+            rotate_eight(x[0], x[1], turn, g.cos != nullptr, k_lo[i], k_hi[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                k_top = fmax(k_top, fmax(fabs(k_lo[i][e]), fabs(k_hi[i][e])));
+                odd = fma(k_lo[i][e], 0.0, fma(k_hi[i][e], 0.0, odd));    // NaN: a value that is not finite
+            }
         }
-        finite = __syncthreads_and(finite);
-        top = block_max(top, lds);
-        const float held = *scale;
-        const bool poisoned = !finite || (slot0 > 0 && held != held);
-        int e = exponent_for(top);
-        int e_held = e;
-        if (slot0 > 0 && !poisoned) {
-            // a power of two as the appends leave it; anything else counts by its exponent
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * PK; ++i)
+        if (i * kTokensV + tid / kUnitsV < tokens) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v_bits = max(v_bits, __float_as_uint(v[i][e]) & 0x7fffffffu);
+        }
+    if (odd != 0.0) k_top = INFINITY;
+    k_top = wave_max(k_top);
+    v_bits = wave_max(v_bits);
+    double v_top = v_bits >= 0x7f800000u ? static_cast<double>(INFINITY) : static_cast<double>(__uint_as_float(v_bits));
+    if constexpr (THREADS > kWave) {
+        if (lane == 0) {
+            lds[0][tid / kWave] = k_top;
+            lds[1][tid / kWave] = v_top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < THREADS / kWave; ++i) {
+            k_top = fmax(k_top, lds[0][i]);
+            v_top = fmax(v_top, lds[1][i]);
+        }
+    }
+    // the step of a block: what its new values need, and what it has if it goes on
+    auto step = [&](double top, float held, int &e_held, bool &marked) {
+        marked = top == static_cast<double>(INFINITY) || (slot0 > 0 && held != held);
+        int e = marked ? 0 : exponent_for(top);
+        e_held = e;
+        if (slot0 > 0 && !marked) {
+            // (a power of two as the appends leave it; anything else counts by its exponent)
             e_held = max(kLowestExponent, min(127, static_cast<int>((__float_as_uint(held) >> 23) & 255u) - 127));
             e = max(e, e_held);
         }
-        if (e > e_held && slot0 > 0) {
-            for (int i = tid; i < slot0 * D; i += kThreads) {
-                int8_t &b = dst[at(i / D, i % D)];
-                b = to_step(static_cast<double>(b), e - e_held);
+        return e;
+    };
+    int k_was, v_was;
+    bool k_marked, v_marked;
+    const int k_e = step(k_top, k_held, k_was, k_marked), v_e = step(v_top, v_held, v_was, v_marked);
+    // values held already, in the new step
+    if (k_e > k_was) {
+        uint32_t *words = reinterpret_cast<uint32_t *>(k_block);
+        const double shrink = power(k_was - k_e);
+        for (int i = tid; i < slot0 * D / 4; i += THREADS) {
+            const uint32_t w = words[i];
+            uint32_t n = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n |= to_byte(static_cast<double>(static_cast<int8_t>(w >> (8 * e))), shrink) << (8 * e);
+            words[i] = n;
+        }
+    }
+    if (v_e > v_was) {
+        const double shrink = power(v_was - v_e);
+        for (int i = tid; i < slot0 * D; i += THREADS) {
+            int8_t &b = v_block[i / slot0 * size + i % slot0];
+            b = static_cast<int8_t>(to_byte(static_cast<double>(b), shrink));
+        }
+    }
+    const double k_inv = k_marked ? 0.0 : power(-k_e);
+    const float v_inv = v_marked ? 0.f : static_cast<float>(power(-v_e));
+#pragma unroll
+    for (int i = 0; i < PK; ++i) {
+        const int t = i * kTokensK + tid / kUnitsK;
+        if (t < tokens) {
+            int8_t *to = k_block + (slot0 + t) * D + unit_k;
+            *reinterpret_cast<uint64_t *>(to) = k_marked ? 0 : to_bytes(k_lo[i], k_inv);
+            *reinterpret_cast<uint64_t *>(to + D / 2) = k_marked ? 0 : to_bytes(k_hi[i], k_inv);
+        }
+    }
+    const bool turn = tokens > 4;
+#pragma unroll
+    for (int i = 0; i < 2 * PK; ++i) {
+        const int t = i * kTokensV + tid / kUnitsV;
+        if (t < tokens) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint8_t b = v_marked ? 0 : static_cast<uint8_t>(to_byte(v[i][e], v_inv));
+                if (turn) turned[unit_v + e][t] = b;
+                else v_block[(unit_v + e) * size + slot0 + t] = static_cast<int8_t>(b);
             }
         }
-        for (int i = tid; i < tokens * D; i += kThreads)
-            dst[at(slot0 + i / D, i % D)] = poisoned ? 0 : to_step(value(i / D, i % D), e);
-        __syncthreads();     // (the scale has been read by every wavefront)
-        if (tid == 0) *scale = poisoned ? __uint_as_float(0x7fc00000u) : ldexpf(1.f, e);
     }
+    if (turn) {
+        __syncthreads();
+        // words of four slots; those at the ends that hold older slots byte by byte
+        const int w0 = slot0 / 4, w1 = (slot1 + 3) / 4;
+        for (int i = tid; i < D * (w1 - w0); i += THREADS) {
+            const int d = i / (w1 - w0), w = w0 + i % (w1 - w0);
+            int8_t *to = v_block + d * size + w * 4;
+            if (w * 4 >= slot0 && w * 4 + 4 <= slot1) {
+                uint32_t n = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) n |= static_cast<uint32_t>(turned[d][w * 4 + e - slot0]) << (8 * e);
+                *reinterpret_cast<uint32_t *>(to) = n;
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (w * 4 + e >= slot0 && w * 4 + e < slot1) to[e] = static_cast<int8_t>(turned[d][w * 4 + e - slot0]);
+            }
+        }
+    }
+    if (tid == 0) {
+        const float nan = __uint_as_float(0x7fc00000u);
+        g.c.k_scale[block] = k_marked ? nan : static_cast<float>(power(k_e));
+        g.c.v_scale[block] = v_marked ? nan : static_cast<float>(power(v_e));
+    }
+}
+
+template <typename T, int D, int THREADS, int PK>
+int32_t launch_append(hipStream_t st, AppendArgs<T> g) {
+    const int64_t q_blocks = (g.q_units + THREADS - 1) / THREADS;
+    const int64_t blocks = static_cast<int64_t>(g.pieces) * g.c.kv_heads + (q_blocks < (1 << 22) ? q_blocks : (1 << 22));
+    paged_append_kernel<T, D, THREADS, PK><<<static_cast<uint32_t>(blocks), THREADS, 0, st>>>(g);
+    return launch_status();
+}
+
+// A wavefront per block where no sequence brings more tokens than it takes in one trip; 256 threads and as many
+// trips as a page needs otherwise.
+template <typename T, int D>
+int32_t launch_append_for(hipStream_t st, const AppendArgs<T> &g) {
+    const int64_t page = static_cast<int64_t>(1) << g.c.page_shift;
+    const int64_t units = (g.c.max_new < page ? g.c.max_new : page) * (D / 16);     // of one block's K at most
+    if (units <= 64) return launch_append<T, D, 64, 1>(st, g);
+    if (units <= 256) return launch_append<T, D, 256, 1>(st, g);
+    if (units <= 512) return launch_append<T, D, 256, 2>(st, g);
+    if constexpr (D == 128) return launch_append<T, D, 256, 4>(st, g);
+    return RMLK_ERR_UNSUPPORTED;      // (128 tokens of 64 dims are 512 units)
 }
 
 }  // namespace
@@ -198,8 +359,6 @@ int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_pa
         return RMLK_ERR_UNSUPPORTED;
     const int64_t pieces = (c.rows >> c.page_shift) + 2 * c.seqs;
     if (pieces * c.kv_heads > (1 << 23)) return RMLK_ERR_TOO_LARGE;
-    const int64_t q_elems = q ? c.rows * heads * d : 0;
-    const int64_t q_blocks = (q_elems + 16 * kThreads - 1) / (16 * kThreads);
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
         AppendArgs<T> g{};
@@ -216,10 +375,8 @@ int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_pa
         g.positions = positions;
         g.heads = static_cast<int32_t>(heads);
         g.pieces = static_cast<int32_t>(pieces);
-        const int64_t blocks = pieces * c.kv_heads + (q_blocks < (1 << 22) ? q_blocks : (1 << 22));
-        if (d == 64) paged_append_kernel<T, 64><<<static_cast<uint32_t>(blocks), kThreads, 0, st>>>(g);
-        else paged_append_kernel<T, 128><<<static_cast<uint32_t>(blocks), kThreads, 0, st>>>(g);
-        return launch_status();
+        g.q_units = q ? c.rows * ((heads + kHeads - 1) / kHeads) * (d / 16) : 0;
+        return d == 64 ? launch_append_for<T, 64>(st, g) : launch_append_for<T, 128>(st, g);
     });
 }
 

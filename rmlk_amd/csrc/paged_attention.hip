@@ -108,18 +108,18 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
     // Blocks of one KV head next to each other would meet on different XCDs (workgroups go round
     // robin): the head is the fastest index, so with eight of them an XCD reads one head's cache. Last
     // row tiles first: they see the most keys.
-    if (!starts_ascend(g.c)) {
-        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
-        return;
-    }
     const int kv = blockIdx.x % g.c.kv_heads;
     const int rest = blockIdx.x / g.c.kv_heads;
     const int split = rest % g.splits;
     const int piece = g.pieces - 1 - rest / g.splits;
-    const int seq = g.one_each ? piece : sequence_of_rows(g.c, piece, g.rep, R);
-    if (seq < 0) return;
+    int seq;
     Sequence s;
-    if (!sequence_at(g.c, seq, s)) {
+    if (!locate(g.c, [&](int32_t first, int i) { return (g.one_each ? 0 : first * g.rep / R) + i <= piece; }, seq, s)) {
+        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
+        return;
+    }
+    if (seq < 0) return;
+    if (!in_bounds(g.c, s)) {
         if (tid == 0) raise_error(g.c);
         return;
     }
@@ -398,14 +398,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
 // The splits of the rows that see more than one: a wavefront per (row, head).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
-    if (!starts_ascend(g.c)) return;
     const int lane = threadIdx.x % kWave;
     const int64_t all_rows = g.c.rows * g.heads;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    if (at >= all_rows) return;
     const int64_t row = at / g.heads;
+    int seq;
     Sequence s;
-    if (!sequence_at(g.c, sequence_of_row(g.c, row), s) || row < s.row || row >= s.row + s.fresh) return;
+    if (!locate(g.c, [&](int32_t first, int) { return first <= row; }, seq, s) || at >= all_rows || seq < 0 ||
+        !in_bounds(g.c, s) || row >= s.row + s.fresh)
+        return;
     const int limit = s.length - s.fresh + static_cast<int>(row - s.row) + 1;
     if (limit <= g.chunk) return;
     const int parts = (limit + g.chunk - 1) / g.chunk;

@@ -12,103 +12,217 @@
 namespace rmlk {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kSmallest = 0x1p-100f;   // rows below it are stored as zeros: 127 / max|y| stays finite
 
-// block-wide sum / max of one value per thread (four wavefronts)
-template <typename T, typename Op>
+template <int THREADS, typename T, typename Op>
 __device__ __forceinline__ T block_reduce(T v, T *lds, Op op) {
+    if constexpr (THREADS == kWave) return v;
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
     __syncthreads();
     T r = lds[0];
 #pragma unroll
-    for (int i = 1; i < kThreads / kWave; ++i) r = op(r, lds[i]);
+    for (int i = 1; i < THREADS / kWave; ++i) r = op(r, lds[i]);
     __syncthreads();
     return r;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int32_t cols,
-                                                                 int8_t *__restrict__ q, int64_t ldq,
-                                                                 float *__restrict__ scale) {
-    __shared__ uint32_t lds[kThreads / kWave];
-    const int64_t row = blockIdx.x;
-    x += row * ldx;
-    q += row * ldq;
-    // magnitudes compare like their bits, NaN and infinity above everything finite
-    uint32_t top = 0;
-    for (int j = threadIdx.x; j < cols; j += kThreads) top = max(top, __float_as_uint(to_float(x[j])) & 0x7fffffffu);
-    top = block_reduce(wave_max(top), lds, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    const float amax = __uint_as_float(top);
-    const bool zero = !(amax >= kSmallest) || top >= 0x7f800000u;
-    const float s = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : zero ? 0.f : amax / 127.f;
-    const float inv = zero ? 0.f : 1.f / s, half = 0.5f * s;
-    const int padded = (cols + 15) & ~15;
-    for (int j = threadIdx.x; j < padded; j += kThreads) {
-        int n = 0;
-        if (j < cols && !zero) {
-            const float v = to_float(x[j]);
-            const float q0 = rintf(v * inv);
-            const float r = fmaf(-q0, s, v);
-            n = static_cast<int>(q0);
-            const float a = fabsf(r);
-            if (a > half || (a == half && (n & 1))) n += r > 0.f ? 1 : -1;
-            n = min(127, max(-127, n));
-        }
-        q[j] = static_cast<int8_t>(n);
+// Eight values of a row from column c on, zeros behind its end. ALIGNED: the row starts at a 16-byte boundary.
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ void load_eight(const T *row, int c, int cols, T (&out)[8]) {
+    if (ALIGNED && c + 8 <= cols) {
+#pragma unroll
+        for (size_t u = 0; u < sizeof(T) / 2; ++u)
+            reinterpret_cast<u32x4 *>(out)[u] = reinterpret_cast<const u32x4 *>(row + c)[u];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = c + e < cols ? row[c + e] : static_cast<T>(0.f);
     }
-    if (threadIdx.x == 0) scale[row] = s;
+}
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ void store_eight(T *row, int c, int cols, const T (&v)[8]) {
+    if (ALIGNED && c + 8 <= cols) {
+#pragma unroll
+        for (size_t u = 0; u < sizeof(T) / 2; ++u)
+            reinterpret_cast<u32x4 *>(row + c)[u] = reinterpret_cast<const u32x4 *>(v)[u];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < cols) row[c + e] = v[e];
+    }
+}
+__device__ __forceinline__ uint64_t pack_eight(const int (&n)[8]) {
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        lo |= static_cast<uint32_t>(n[e] & 255) << (8 * e);
+        hi |= static_cast<uint32_t>(n[4 + e] & 255) << (8 * e);
+    }
+    return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_quantize_kernel(const T *x, const T *b, const float *__restrict__ gamma,
-                                                                 float eps, int32_t cols, T *sum_out,
-                                                                 int8_t *__restrict__ q, int64_t ldq,
-                                                                 float *__restrict__ scale) {
-    __shared__ double lds_d[kThreads / kWave];
-    __shared__ uint64_t lds_u[kThreads / kWave];
-    const int64_t row = blockIdx.x;
-    x += row * cols;
-    q += row * ldq;
-    if (b) {
-        b += row * cols;
-        sum_out += row * cols;
-    }
-    double square = 0.0;
-    for (int j = threadIdx.x; j < cols; j += kThreads) {
-        float v = to_float(x[j]);
-        if (b) {
-            const T t = static_cast<T>(v + to_float(b[j]));
-            sum_out[j] = t;
-            v = to_float(t);
+// A block per row, which it holds in registers: CH units of eight values per thread, one pass over memory.
+// CH = 0: a row of any length, read twice (the second time from the caches).
+template <typename T, int THREADS, int CH, bool ALIGNED>
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T *__restrict__ xs, int64_t ldx, int64_t rows,
+                                                                int32_t cols, int8_t *__restrict__ qs, int64_t ldq,
+                                                                float *__restrict__ scale) {
+    __shared__ uint32_t lds[THREADS / kWave];
+    const int padded = (cols + 15) & ~15, tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *x = xs + row * ldx;
+        int8_t *q = qs + row * ldq;
+        T held[CH > 0 ? CH : 1][8];
+        // magnitudes compare like their bits, NaN and infinity above everything finite
+        uint32_t top = 0;
+        auto magnitude = [&](const T (&v)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(to_float(v[e])) & 0x7fffffffu);
+        };
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) load_eight<ALIGNED>(x, (i * THREADS + tid) * 8, cols, held[i]);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) magnitude(held[i]);
+        } else {
+            for (int c = tid * 8; c < cols; c += THREADS * 8) {
+                load_eight<ALIGNED>(x, c, cols, held[0]);
+                magnitude(held[0]);
+            }
         }
-        square += static_cast<double>(v) * static_cast<double>(v);
+        top = block_reduce<THREADS>(wave_max(top), lds, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        const float amax = __uint_as_float(top);
+        const bool zero = !(amax >= kSmallest) || top >= 0x7f800000u;
+        const float s = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : zero ? 0.f : amax / 127.f;
+        const float inv = zero ? 0.f : 1.f / s, half = 0.5f * s;
+        auto quantize = [&](const T (&v)[8], int c) {
+            int n[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = to_float(v[e]), q0 = rintf(y * inv), r = fmaf(-q0, s, y), a = fabsf(r);
+                n[e] = static_cast<int>(q0);
+                if (a > half || (a == half && (n[e] & 1))) n[e] += r > 0.f ? 1 : -1;
+                n[e] = zero ? 0 : min(127, max(-127, n[e]));
+            }
+            *reinterpret_cast<uint64_t *>(q + c) = pack_eight(n);
+        };
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (const int c = (i * THREADS + tid) * 8; c < padded) quantize(held[i], c);
+        } else {
+            for (int c = tid * 8; c < padded; c += THREADS * 8) {
+                load_eight<ALIGNED>(x, c, cols, held[0]);
+                quantize(held[0], c);
+            }
+        }
+        if (tid == 0) scale[row] = s;
     }
-    square = block_reduce(wave_sum(square), lds_d, [](double a, double c) { return a + c; });
-    const double factor = 1.0 / sqrt(square / cols + static_cast<double>(eps));
-    const T *y = b ? sum_out : x;     // (every thread reads back what it wrote itself)
-    uint64_t top = 0;
-    for (int j = threadIdx.x; j < cols; j += kThreads) {
-        const double v = to_float(y[j]) * factor * static_cast<double>(gamma[j]);
-        const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v)) & 0x7fffffffffffffffull;
-        top = u > top ? u : top;
-    }
-    top = block_reduce(wave_max(top), lds_u, [](uint64_t a, uint64_t c) { return a > c ? a : c; });
-    const double amax = __longlong_as_double(static_cast<long long>(top));
-    const float s_of = static_cast<float>(amax / 127.0);
-    const bool bad = !(s_of <= 3.402823466e38f);   // NaN, infinite, or beyond what a scale can hold
-    const bool zero = bad || amax < static_cast<double>(kSmallest);
-    const float s = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.f : s_of;
-    const double inv = zero ? 0.0 : 1.0 / static_cast<double>(s);
-    const int padded = (cols + 15) & ~15;
-    for (int j = threadIdx.x; j < padded; j += kThreads) {
-        int n = 0;
-        if (j < cols && !zero)
-            n = static_cast<int>(rint(to_float(y[j]) * factor * static_cast<double>(gamma[j]) * inv));
-        q[j] = static_cast<int8_t>(min(127, max(-127, n)));
-    }
-    if (threadIdx.x == 0) scale[row] = s;
 }
+
+// The same behind RMSNorm: y = x * f * gamma with f = 1 / sqrt(mean(x^2) + eps). A thread holds the exact
+// products x * gamma (48 bits) in double; their largest magnitude times f is the row's, and
+// y / scale = x * gamma * (f / scale).
+template <typename T, int THREADS, int CH, bool ALIGNED>
+__global__ __launch_bounds__(THREADS) void norm_quantize_kernel(const T *xs, const T *bs, const float *__restrict__ gamma,
+                                                                float eps, int64_t rows, int32_t cols, T *sums,
+                                                                int8_t *__restrict__ qs, int64_t ldq,
+                                                                float *__restrict__ scale) {
+    __shared__ double lds[THREADS / kWave], lds2[THREADS / kWave], lds3[THREADS / kWave];
+    const int padded = (cols + 15) & ~15, tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *x = xs + row * cols, *b = bs ? bs + row * cols : nullptr;
+        T *sum = bs ? sums + row * cols : nullptr;
+        int8_t *q = qs + row * ldq;
+        double held[CH > 0 ? CH : 1][8], square = 0.0, top = 0.0, odd = 0.0;
+        // loads a unit, forms the sum where there is one, adds up squares, leaves the products in p
+        auto products = [&](int c, double (&p)[8], const T (&v)[8], const T (&w)[8], const float (&gm)[8]) {
+            T t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                t[e] = v[e];
+                if (b) t[e] = static_cast<T>(to_float(v[e]) + to_float(w[e]));
+                const double y = to_float(t[e]);
+                square = fma(y, y, square);
+                p[e] = y * static_cast<double>(gm[e]);
+                top = fmax(top, fabs(p[e]));
+                odd = fma(p[e], 0.0, odd);       // NaN with the first product that is not finite
+            }
+            if (b && c < cols) store_eight<ALIGNED>(sum, c, cols, t);
+        };
+        if constexpr (CH > 0) {
+            T v[CH][8], w[CH][8];
+            float gm[CH][8];
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int c = (i * THREADS + tid) * 8;
+                load_eight<ALIGNED>(x, c, cols, v[i]);
+                if (b) load_eight<ALIGNED>(b, c, cols, w[i]);
+                load_eight<ALIGNED>(gamma, c, cols, gm[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) products((i * THREADS + tid) * 8, held[i], v[i], w[i], gm[i]);
+        } else {
+            for (int c = tid * 8; c < cols; c += THREADS * 8) {
+                T v[8], w[8];
+                float gm[8];
+                load_eight<ALIGNED>(x, c, cols, v);
+                if (b) load_eight<ALIGNED>(b, c, cols, w);
+                load_eight<ALIGNED>(gamma, c, cols, gm);
+                products(c, held[0], v, w, gm);
+            }
+        }
+        auto add = [](double a, double c) { return a + c; };
+        square = block_reduce<THREADS>(wave_sum(square), lds, add);
+        odd = block_reduce<THREADS>(wave_sum(odd), lds2, add);
+        top = block_reduce<THREADS>(wave_max(top), lds3, [](double a, double c) { return c > a ? c : a; });
+        const double f = 1.0 / sqrt(square / cols + static_cast<double>(eps));
+        const double amax = top * f;
+        const float s_of = static_cast<float>(amax / 127.0);
+        // (infinite squares, an infinite or NaN product, a scale beyond float)
+        const bool bad = !(odd == 0.0) || !(square <= 1.7976931348623157e308) || !(s_of <= 3.402823466e38f);
+        const bool zero = bad || amax < static_cast<double>(kSmallest);
+        const float s = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.f : s_of;
+        const double to_step = zero ? 0.0 : f / static_cast<double>(s);
+        auto quantize = [&](const double (&p)[8], int c) {
+            int n[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) n[e] = zero ? 0 : min(127, max(-127, static_cast<int>(rint(p[e] * to_step))));
+            *reinterpret_cast<uint64_t *>(q + c) = pack_eight(n);
+        };
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (const int c = (i * THREADS + tid) * 8; c < padded) quantize(held[i], c);
+        } else {
+            for (int c = tid * 8; c < padded; c += THREADS * 8) {
+                T v[8];
+                float gm[8];
+                load_eight<ALIGNED>(b ? sum : x, c, cols, v);      // (every thread reads back what it wrote itself)
+                load_eight<ALIGNED>(gamma, c, cols, gm);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) held[0][e] = static_cast<double>(to_float(v[e])) * static_cast<double>(gm[e]);
+                quantize(held[0], c);
+            }
+        }
+        if (tid == 0) scale[row] = s;
+    }
+}
+
+// f(threads, units per thread) as constants: a wavefront for short rows, larger blocks for longer ones, rows of
+// up to 16384 values held in registers. MOST: units a thread may hold (the norm's take 40 registers each).
+template <int MOST, typename F>
+int32_t with_row_shape(int32_t cols, F &&f) {
+    using std::integral_constant;
+    const int units = (cols + 15) / 16 * 2;
+    if (units <= 64) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (units <= 256) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    if (units <= 512) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    constexpr int kFour = MOST >= 4 ? 256 : 512, kEight = MOST >= 8 ? 256 : 1024;
+    if (units <= 1024) return f(integral_constant<int, kFour>{}, integral_constant<int, 1024 / kFour>{});
+    if (units <= 2048) return f(integral_constant<int, kEight>{}, integral_constant<int, 2048 / kEight>{});
+    return f(integral_constant<int, 256>{}, integral_constant<int, 0>{});
+}
+inline uint32_t row_blocks(int64_t rows) { return static_cast<uint32_t>(rows < (1 << 20) ? rows : (1 << 20)); }
 
 int32_t row_checks(int32_t dtype, int64_t rows, int64_t cols, const void *q, int64_t ldq) {
     if (rows < 0 || cols < 0) return RMLK_ERR_INVALID_ARGUMENT;
@@ -135,9 +249,14 @@ int32_t rmlk_hip_quantize_rows(rmlk_stream_t stream, int32_t dtype, int64_t rows
     if (!x || !q || !scale) return RMLK_ERR_NULL_POINTER;
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
-        quantize_rows_kernel<T><<<static_cast<uint32_t>(rows), kThreads, 0, st>>>(
-            static_cast<const T *>(x), ldx, static_cast<int32_t>(cols), static_cast<int8_t *>(q), ldq, scale);
-        return launch_status();
+        const bool aligned = aligned16(x) && ldx * sizeof(T) % 16 == 0;
+        return with_row_shape<8>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
+            constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
+            auto kern = aligned ? quantize_rows_kernel<T, THREADS, CH, true> : quantize_rows_kernel<T, THREADS, CH, false>;
+            kern<<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), ldx, rows, static_cast<int32_t>(cols),
+                                                        static_cast<int8_t *>(q), ldq, scale);
+            return launch_status();
+        });
     });
 }
 
@@ -150,10 +269,16 @@ int32_t rmlk_hip_rmsnorm_quantize_rows(rmlk_stream_t stream, int32_t dtype, int6
     if (!x || !gamma || !q || !scale || (b == nullptr) != (sum_out == nullptr)) return RMLK_ERR_NULL_POINTER;
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
-        norm_quantize_kernel<T><<<static_cast<uint32_t>(rows), kThreads, 0, st>>>(
-            static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps, static_cast<int32_t>(cols),
-            static_cast<T *>(sum_out), static_cast<int8_t *>(q), ldq, scale);
-        return launch_status();
+        const bool aligned = cols * sizeof(T) % 16 == 0 && cols % 4 == 0 && aligned16(x) && aligned16(b) &&
+                             aligned16(sum_out) && aligned16(gamma);
+        return with_row_shape<2>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
+            constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
+            auto kern = aligned ? norm_quantize_kernel<T, THREADS, CH, true> : norm_quantize_kernel<T, THREADS, CH, false>;
+            kern<<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps,
+                                                        rows, static_cast<int32_t>(cols), static_cast<T *>(sum_out),
+                                                        static_cast<int8_t *>(q), ldq, scale);
+            return launch_status();
+        });
     });
 }
 
