@@ -1,18 +1,16 @@
 // Attention over the paged int8 cache: out = Softmax(q . K^T * scale) . V per sequence, a query seeing the
 // tokens up to its own position; prompts, chunks of prompts and single tokens alike.
 //
-// The rows of one KV head (its rep query heads times the sequence's new tokens) form one matrix. A
-// block takes 16 * NT of them; its wavefronts share them and deal the keys out among themselves in
-// tiles of 64, each with its own running maximum, sum and output, which meet in LDS at the end. Long
-// caches are split over several blocks besides, whose normalised results a second kernel joins.
+// The rows of one KV head (its rep query heads times the sequence's new tokens) form one matrix, cut into
+// tiles of rows. Long caches are split over several blocks besides, whose normalised results a second
+// kernel joins.
 //
 // Everything is computed transposed, so that a query stays in one lane column from its scores to its
 // output: S^T = K . Q^T by v_mfma_f32_16x16x32_f16 leaves four keys of a query in a lane, and the keys
 // of a tile are assigned to the rows of the four S^T blocks such that a lane's sixteen weights belong to
 // sixteen CONSECUTIVE tokens (16 g .. 16 g + 15 for lane group g): they are the B operand of
 // O^T += V^T . P^T as they are, and the A operand is sixteen consecutive bytes of a row of the transposed
-// V block. No score, weight or cache value passes through LDS; K and V go from memory to registers in
-// 16-byte loads, one tile ahead.
+// V block. No score or weight passes through LDS; K and V come from memory in 16-byte loads, one tile ahead.
 //
 // int8 -> half: a byte b with its sign bit flipped, u = b + 128, under the high byte 0x64 is the half
 // 1024 + u; one packed add of -1152 gives b (K), one packed fma (1024 + u) * f - 1152 f gives b * f
@@ -34,11 +32,13 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileKeys = 64;
 constexpr float kBase = 7.f;          // log2 of the weight of a key that scores the reference maximum
+constexpr float kLeastFactor = 1.17549435e-38f;
 constexpr float kMostWeight = 15.f;   // log2 of the largest weight before the reference point moves
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
 struct AttendArgs {
@@ -97,101 +97,274 @@ struct Tile {
     bool bad;            // the page lies outside the cache
 };
 
+// Sixteen NT rows of a wavefront's lane columns: what they see and their queries as halves.
+template <typename T, int D, int NT>
+struct Rows {
+    static constexpr int P = sizeof(T) == 4 ? 2 : 1;   // half pieces of a query value and of a weight
+    static constexpr int KH = D / 32;
+    int limit[NT];             // tokens the row sees
+    float factor[NT];          // of a score but for K's step
+    h8 q[P][NT][KH];
+
+    // rows r0 .. of the `rows` of one KV head of a sequence
+    __device__ __forceinline__ void load(const AttendArgs<T> &g, const Sequence &s, int kv, int r0, int rows) {
+        const int lane = threadIdx.x % kWave, col = lane % 16, grp = lane / 16;
+        const int past = s.length - s.fresh;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = r0 + n * 16 + col;
+            const bool live = r < rows;
+            limit[n] = live ? past + r / g.rep + 1 : 0x7fffffff;   // (a row that is not there: no mask, zeros)
+            float x[D / 64][16];
+            const T *src = g.q + (s.row + (live ? r / g.rep : 0)) * g.q_stride +
+                           static_cast<int64_t>(kv * g.rep + (live ? r % g.rep : 0)) * D + grp * 16;
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                load_row(src + c * 64, x[c]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (!live) x[c][i] = 0.f;
+                    const uint32_t bits = __float_as_uint(x[c][i]) & 0x7fffffffu;
+                    top = bits > top ? bits : top;
+                }
+            }
+            uint32_t other = __shfl_xor(top, 16, kWave);
+            top = other > top ? other : top;
+            other = __shfl_xor(top, 32, kWave);
+            top = other > top ? other : top;
+            const int e = max(-113, static_cast<int>(top >> 23) - 127);
+            // (the scale's sign goes to the query: factors are positive)
+            const float up = copysignf(__uint_as_float(static_cast<uint32_t>(13 - e + 127) << 23), g.scale);
+            factor[n] = __uint_as_float(static_cast<uint32_t>(e - 13 + 127) << 23) * fabsf(g.scale);
+            if (top >= 0x7f800000u) factor[n] = __uint_as_float(0x7fc00000u);   // (an infinity or a NaN in the row)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float v = x[c][h * 8 + j] * up;
+                        const _Float16 hi = static_cast<_Float16>(v);
+                        q[0][n][c * 2 + h][j] = hi;
+                        if constexpr (P == 2) q[1][n][c * 2 + h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
+                    }
+        }
+    }
+};
+
+// What a wavefront has of its rows' softmax: outputs (times 2^-E), sums, reference points.
+template <typename T, int D, int NT>
+struct Softmax {
+    static constexpr int P = Rows<T, D, NT>::P, DT = D / 16, KH = D / 32;
+    f32x4 acc[DT][NT];
+    float sum[NT], ref[NT];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            sum[n] = 0.f;
+            ref[n] = -3.402823466e38f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    __device__ __forceinline__ void rescale(float f) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[d][n] *= f;
+    }
+    // One tile: k_frag(jj, h) and v_frag(d, hh) give the operands, kc K's step of the lane group's tokens;
+    // t0 the tile's first token, masked whether any row of the wavefront does not see all of it, bad whether the
+    // lane group's tokens are hidden from everyone. A hidden score becomes -inf before it is scaled: factors
+    // are kept positive, and where a row sees none of the lane group's tokens its factor is replaced, so that
+    // a step that is no number reaches only the rows that see the block.
+    template <typename KF, typename VF>
+    __device__ __forceinline__ void tile(const Rows<T, D, NT> &rows, KF &&k_frag, VF &&v_frag, float kc, int t0,
+                                         bool masked, bool bad) {
+        const int grp = threadIdx.x % kWave / 16;
+        float c[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            c[n] = rows.factor[n] * kc;
+            c[n] = c[n] < kLeastFactor ? kLeastFactor : c[n];
+        }
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) c[n] = rows.limit[n] <= t0 + grp * 16 || bad ? kLeastFactor : c[n];
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            f32x4 sc[2][NT];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < KH; ++q) {
+                    const h8 kf = k_frag(2 * hh + j, q);
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, rows.q[p][n][q], sc[j][n], 0, 0, 0);
+                }
+            }
+            if (masked) {
+                const int key = t0 + grp * 16 + hh * 8;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        sc[i / 4][n][i % 4] = key + i < rows.limit[n] && !bad ? sc[i / 4][n][i % 4] : -INFINITY;
+            }
+            // exponents relative to the reference point (which is finite: a hidden score stays -inf)
+            auto exponent = [&](int n, int i) { return fmaf(sc[i / 4][n][i % 4], c[n], -ref[n]); };
+            bool beyond = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, exponent(n, i));
+                beyond = top > kMostWeight || beyond;
+            }
+            if (__any(beyond)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[i / 4][n][i % 4] * c[n]);
+                    const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
+                    const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
+                    ref[n] = now;
+                    sum[n] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
+                }
+            }
+            h8 pf[P][NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const f32x2 w = {__builtin_amdgcn_exp2f(exponent(n, i)), __builtin_amdgcn_exp2f(exponent(n, i + 1))};
+                    sum[n] += w[0];
+                    sum[n] += w[1];
+                    const h2 hi = __builtin_convertvector(w, h2);
+                    pf[0][n][i] = hi[0];
+                    pf[0][n][i + 1] = hi[1];
+                    if constexpr (P == 2) {
+                        const f32x2 rest = {w[0] - static_cast<float>(hi[0]), w[1] - static_cast<float>(hi[1])};
+                        const h2 lo = __builtin_convertvector(rest, h2);
+                        pf[1][n][i] = lo[0];
+                        pf[1][n][i + 1] = lo[1];
+                    }
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const h8 va = v_frag(d, hh);
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// log2 of the largest step of V among the four lane groups' pages; a step that is no number counts as none.
+__device__ __forceinline__ int largest_step(float v_scale, bool odd) {
+    int e = odd ? -127 : static_cast<int>((__float_as_uint(v_scale) >> 23) & 255u) - 127;
+    return max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
+               max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(T *to, const f32x4 &o) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4 *>(to) = o;
+    } else {
+        T v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(o[e]);
+        *reinterpret_cast<u32x2 *>(to) = *reinterpret_cast<u32x2 *>(v);
+    }
+}
+
+// Four neighbouring outputs of a row: the result, or (more than one split) a part of it with its statistics.
+template <typename T, int D>
+__device__ __forceinline__ void put_output(const AttendArgs<T> &g, const Sequence &s, int kv, int r, int split, int d,
+                                           const f32x4 &o, float ref, float total) {
+    const int token = r / g.rep;
+    const int64_t at = (s.row + token) * static_cast<int64_t>(g.heads) + kv * g.rep + r % g.rep;
+    if (s.length - s.fresh + token + 1 <= g.chunk) {     // (all it sees lies in the first split)
+        if (split == 0) store_four(g.out + at * D + d, o);
+    } else {
+        const int64_t all_rows = g.c.rows * g.heads;
+        *reinterpret_cast<f32x4 *>(g.part + (split * all_rows + at) * D + d) = o;
+        if (d == 0)
+            reinterpret_cast<float2 *>(g.part + g.splits * all_rows * D)[split * all_rows + at] = float2{ref, total};
+    }
+}
+
+// The place of a block in the work: KV head, sequence, first row, split. False: nothing to do.
+struct Place {
+    int kv, seq, split, r0, rows, most, least, begin, end;
+    Sequence s;
+};
+template <typename T>
+__device__ __forceinline__ bool find_place(const AttendArgs<T> &g, int tile_rows, Place &p) {
+    // Blocks of one KV head next to each other would meet on different XCDs (workgroups go round robin): the
+    // head is the fastest index, so with eight of them an XCD reads one head's cache. Last row tiles first:
+    // they see the most keys.
+    p.kv = blockIdx.x % g.c.kv_heads;
+    const int rest = blockIdx.x / g.c.kv_heads;
+    p.split = rest % g.splits;
+    const int piece = g.pieces - 1 - rest / g.splits;
+    if (!locate(g.c, [&](int32_t first, int i) { return (g.one_each ? 0 : first * g.rep / tile_rows) + i <= piece; }, p.seq,
+                p.s)) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(g.c);
+        return false;
+    }
+    if (p.seq < 0) return false;
+    if (!in_bounds(g.c, p.s)) {
+        if (threadIdx.x == 0) raise_error(g.c);
+        return false;
+    }
+    const int index = g.one_each ? 0 : piece - (p.s.row * g.rep / tile_rows + p.seq);
+    p.rows = p.s.fresh * g.rep;
+    p.r0 = index * tile_rows;
+    if (index < 0 || p.r0 >= p.rows) return false;
+    const int past = p.s.length - p.s.fresh;           // position of the sequence's first row
+    p.most = past + min(p.r0 + tile_rows - 1, p.rows - 1) / g.rep + 1;   // tokens the last row sees
+    p.least = past + p.r0 / g.rep + 1;
+    p.begin = p.split * g.chunk;
+    if (p.split > 0 && p.begin >= p.most) return false;
+    p.end = min(p.most, p.begin + g.chunk);
+    return true;
+}
+
+// Few rows (16 * NT of them): the wavefronts of a block deal the tiles of keys out among themselves, everything
+// in registers.
 template <typename T, int D, int NT, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g) {
-    constexpr int P = sizeof(T) == 4 ? 2 : 1;      // half pieces of a query value and of a weight
+__global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<T> g) {
     constexpr int DT = D / 16, KC = D / 64, R = 16 * NT, kPad = D + 4;
     extern __shared__ __align__(16) float lds[];   // [WAVES][R][kPad], then (max, sum) [WAVES][R]
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % 16, grp = lane / 16;
-
-    // Blocks of one KV head next to each other would meet on different XCDs (workgroups go round
-    // robin): the head is the fastest index, so with eight of them an XCD reads one head's cache. Last
-    // row tiles first: they see the most keys.
-    const int kv = blockIdx.x % g.c.kv_heads;
-    const int rest = blockIdx.x / g.c.kv_heads;
-    const int split = rest % g.splits;
-    const int piece = g.pieces - 1 - rest / g.splits;
-    int seq;
-    Sequence s;
-    if (!locate(g.c, [&](int32_t first, int i) { return (g.one_each ? 0 : first * g.rep / R) + i <= piece; }, seq, s)) {
-        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
-        return;
-    }
-    if (seq < 0) return;
-    if (!in_bounds(g.c, s)) {
-        if (tid == 0) raise_error(g.c);
-        return;
-    }
-    const int index = g.one_each ? 0 : piece - (s.row * g.rep / R + seq);
-    const int rows = s.fresh * g.rep, r0 = index * R;
-    if (index < 0 || r0 >= rows) return;
-    const int past = s.length - s.fresh;           // position of the sequence's first row
-    const int most = past + min(r0 + R - 1, rows - 1) / g.rep + 1;   // tokens the last row sees
-    const int least = past + r0 / g.rep + 1;
-    const int begin = split * g.chunk;
-    if (split > 0 && begin >= most) return;
-    const int end = min(most, begin + g.chunk);
-
-    // the rows of this lane column: what they see, their query as halves
-    int limit[NT];
-    float factor[NT];          // of an S^T element but for K's step
-    h8 qf[P][NT][2 * KC];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = r0 + n * 16 + col;
-        const bool live = r < rows;
-        limit[n] = live ? past + r / g.rep + 1 : 0x7fffffff;   // (a row that is not there: no mask, zeros)
-        float x[KC][16];
-        const T *src = g.q + (s.row + (live ? r / g.rep : 0)) * g.q_stride +
-                       static_cast<int64_t>(kv * g.rep + (live ? r % g.rep : 0)) * D + grp * 16;
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            load_row(src + c * 64, x[c]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (!live) x[c][i] = 0.f;
-                const uint32_t bits = __float_as_uint(x[c][i]) & 0x7fffffffu;
-                top = bits > top ? bits : top;
-            }
-        }
-        uint32_t other = __shfl_xor(top, 16, kWave);
-        top = other > top ? other : top;
-        other = __shfl_xor(top, 32, kWave);
-        top = other > top ? other : top;
-        // (an infinity or a NaN in the row: the factor is whatever, the products are NaN)
-        const int e = max(-113, static_cast<int>(top >> 23) - 127);
-        const float up = __uint_as_float(static_cast<uint32_t>(13 - e + 127) << 23);
-        factor[n] = __uint_as_float(static_cast<uint32_t>(e - 13 + 127) << 23) * g.scale;
-        if (top >= 0x7f800000u) factor[n] = __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = x[c][h * 8 + j] * up;
-                    const _Float16 hi = static_cast<_Float16>(v);
-                    qf[0][n][c * 2 + h][j] = hi;
-                    if constexpr (P == 2) qf[1][n][c * 2 + h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
-                }
-    }
-
-    f32x4 acc[DT][NT];
-    float sum[NT], ref[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        sum[n] = 0.f;
-        ref[n] = -INFINITY;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    Place p;
+    if (!find_place(g, R, p)) return;
+    Rows<T, D, NT> rows;
+    rows.load(g, p.s, p.kv, p.r0, p.rows);
+    Softmax<T, D, NT> soft;
+    soft.clear();
     int step_exp = -200;       // E: log2 of the largest step of V met so far
 
-    const int last_page = (s.length > 0 ? s.length - 1 : 0) >> g.c.page_shift;
+    const int last_page = (p.s.length > 0 ? p.s.length - 1 : 0) >> g.c.page_shift;
     const int size = 1 << g.c.page_shift;
-    const int32_t *table = g.c.table + seq * g.c.table_stride;
+    const int32_t *table = g.c.table + p.seq * g.c.table_stride;
     // pages of the tokens whose K rows (by lane column) and whose V columns (by lane group) a lane loads
     auto pages_of = [&](int t0, int32_t &pk, int32_t &pv) {
         pk = table[min((t0 + (col / 4) * 16) >> g.c.page_shift, last_page)];
@@ -202,7 +375,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
         if (t.bad) raise_error(g.c);
         pk = pk < 0 || pk >= g.c.pages ? 0 : pk;
         pv = t.bad ? 0 : pv;
-        const int64_t bk = (static_cast<int64_t>(pk) * g.c.kv_heads + kv), bv = static_cast<int64_t>(pv) * g.c.kv_heads + kv;
+        const int64_t bk = static_cast<int64_t>(pk) * g.c.kv_heads + p.kv, bv = static_cast<int64_t>(pv) * g.c.kv_heads + p.kv;
         const int8_t *k = g.c.k + (bk * size + ((t0 + (col / 4) * 16 + col % 4) & (size - 1))) * D + grp * 16;
         const int8_t *v = g.c.v + bv * size * D + ((t0 + grp * 16) & (size - 1)) + static_cast<int64_t>(col) * size;
         t.k_scale = g.c.k_scale[bv];
@@ -215,126 +388,45 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
         for (int d = 0; d < DT; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + static_cast<int64_t>(d) * 16 * size);
     };
     auto compute = [&](const Tile<D> &t, int t0) {
-        const bool masked = t0 + kTileKeys > least || __any(t.bad);
         // V's steps relative to the largest; a step that is no number marks the scores instead
-        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f);
-        const float vs = odd || t.bad ? 0.f : t.v_scale;
-        int e = static_cast<int>((__float_as_uint(vs) >> 23) & 255u) - 127;
-        e = max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
-                max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
+        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
+        const int e = largest_step(t.v_scale, odd);
         if (e > step_exp) {
-            const float down = ldexpf(1.f, step_exp - e);
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[d][n] *= down;
+            soft.rescale(ldexpf(1.f, step_exp - e));
             step_exp = e;
         }
-        const _Float16 f1 = static_cast<_Float16>(ldexpf(vs, -step_exp));
+        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
         const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
         const h2 vf = {f1, f1}, vbias = {b1, b1};
         const float kc = odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale;
-        float c[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) c[n] = factor[n] * kc;
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            f32x4 sc[2][NT];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) sc[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int q = 0; q < 2 * KC; ++q) {
-                    const u32x4 raw = t.k[2 * hh + j][q / 2];
-                    const h8 kf = q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
-#pragma unroll
-                    for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[p][n][q], sc[j][n], 0, 0, 0);
-                }
-            }
-            // exponents relative to the reference point
-            const int key = t0 + grp * 16 + hh * 8;
-            auto exponents = [&](int n, float (&x)[8]) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v = fmaf(sc[j][n][i], c[n], -ref[n]);
-                        if (masked) v = key + j * 4 + i < limit[n] && !t.bad ? v : -INFINITY;
-                        x[j * 4 + i] = v;
-                        top = fmaxf(top, v);
-                    }
-                return top;
-            };
-            float x[NT][8];
-            bool beyond = false;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) beyond = exponents(n, x[n]) > kMostWeight || beyond;
-            if (__any(beyond)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool see = !masked || (key + j * 4 + i < limit[n] && !t.bad);
-                            top = fmaxf(top, see ? sc[j][n][i] * c[n] : -INFINITY);
-                        }
-                    const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
-                    const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
-                    ref[n] = now;
-                    sum[n] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
-                    exponents(n, x[n]);
-                }
-            }
-            h8 pf[P][NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(x[n][i]);
-                    sum[n] += w;
-                    const _Float16 hi = static_cast<_Float16>(w);
-                    pf[0][n][i] = hi;
-                    if constexpr (P == 2) pf[1][n][i] = static_cast<_Float16>(w - static_cast<float>(hi));
-                }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const h8 va = widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias);
-#pragma unroll
-                for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
-            }
-        }
+        soft.tile(
+            rows,
+            [&](int j, int q) {
+                const u32x4 raw = t.k[j][q / 2];
+                return q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
+            },
+            [&](int d, int hh) { return widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias); }, kc, t0,
+            t0 + kTileKeys > p.least || __any(t.bad), t.bad);
     };
 
     // tiles begin + 64 * (wave + i * WAVES): the next one is on its way while one is computed, the page
     // numbers of the one after that besides
     constexpr int kStride = kTileKeys * WAVES;
-    int t0 = begin + wave * kTileKeys;
-    if (t0 < end) {
+    int t0 = p.begin + wave * kTileKeys;
+    if (t0 < p.end) {
         Tile<D> one, two;
         int32_t pk, pv;
         pages_of(t0, pk, pv);
         int32_t next_pk = 0, next_pv = 0;
-        if (t0 + kStride < end) pages_of(t0 + kStride, next_pk, next_pv);
+        if (t0 + kStride < p.end) pages_of(t0 + kStride, next_pk, next_pv);
         fetch(one, t0, pk, pv);
         while (true) {
             auto half_step = [&](Tile<D> &now, Tile<D> &next) {
                 const int t1 = t0 + kStride, t2 = t1 + kStride;
-                const bool more = t1 < end;
+                const bool more = t1 < p.end;
                 if (more) {
                     const int32_t a = next_pk, b = next_pv;
-                    if (t2 < end) pages_of(t2, next_pk, next_pv);
+                    if (t2 < p.end) pages_of(t2, next_pk, next_pv);
                     fetch(next, t1, a, b);
                 }
                 compute(now, t0);
@@ -350,23 +442,21 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
     float2 *stats = reinterpret_cast<float2 *>(lds + WAVES * R * kPad);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const float total = across_groups_sum(sum[n]);
+        const float total = across_groups_sum(soft.sum[n]);
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        if (grp == 0) stats[wave * R + n * 16 + col] = float2{ref[n], total};
+        if (grp == 0) stats[wave * R + n * 16 + col] = float2{soft.ref[n], total};
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            f32x4 o = acc[d][n] * inv;
+            f32x4 o = soft.acc[d][n] * inv;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], step_exp);
             *reinterpret_cast<f32x4 *>(lds + (wave * R + n * 16 + col) * kPad + d * 16 + grp * 4) = o;
         }
     }
     __syncthreads();
-    const int64_t all_rows = g.c.rows * g.heads;
     for (int i = tid; i < R * (D / 4); i += WAVES * kWave) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
-        const int r = r0 + row;
-        if (r >= rows) break;
+        if (p.r0 + row >= p.rows) break;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w * R + row].x);
@@ -380,17 +470,135 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_kernel(AttendArgs<T> g
             o += *reinterpret_cast<const f32x4 *>(lds + (w * R + row) * kPad + d) * weight;
         }
         o *= total == 0.f ? 0.f : 1.f / total;
-        const int64_t at = (s.row + r / g.rep) * static_cast<int64_t>(g.heads) + kv * g.rep + r % g.rep;
-        if (past + r / g.rep + 1 <= g.chunk) {     // (all it sees lies in the first split)
-            if (split == 0) {
-                T *dst = g.out + at * D + d;
+        put_output<T, D>(g, p.s, p.kv, p.r0 + row, p.split, d, o, top, total);
+    }
+}
+
+// Many rows: four wavefronts of 16 * NT rows each walk the same tiles of keys. A wavefront fetches and widens a
+// quarter of a tile and leaves it in LDS as the MFMA operands it is (64 lanes x 16 bytes each, read back as
+// they were written: no bank conflicts); two buffers, one barrier per tile. What widening costs, and the
+// trips to the caches, are shared by the block's rows.
+constexpr int kManyWaves = 4;
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(AttendArgs<T> g) {
+    constexpr int DT = D / 16, KC = D / 64, KH = D / 32, R = 16 * NT * kManyWaves, DW = DT / kManyWaves;
+    constexpr int kFrags = 4 * KH + 2 * DT;        // of a tile: K's [4][KH], then V's [DT][2]
+    extern __shared__ __align__(16) u32x4 frags[];   // [2][kFrags][64 lanes]
+    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int col = lane % 16, grp = lane / 16;
+    Place p;
+    if (!find_place(g, R, p)) return;
+    const int my_r0 = p.r0 + wave * 16 * NT;
+    Rows<T, D, NT> rows;
+    rows.load(g, p.s, p.kv, my_r0, p.rows);
+    Softmax<T, D, NT> soft;
+    soft.clear();
+    const int past = p.s.length - p.s.fresh;
+    const int my_least = past + my_r0 / g.rep + 1;
+    const int my_end = my_r0 < p.rows ? min(p.end, past + min(my_r0 + 16 * NT - 1, p.rows - 1) / g.rep + 1) : 0;
+
+    const int last_page = (p.s.length > 0 ? p.s.length - 1 : 0) >> g.c.page_shift;
+    const int size = 1 << g.c.page_shift;
+    const int32_t *table = g.c.table + p.seq * g.c.table_stride;
+    // a quarter of a tile: the K rows of one S^T block, DW row blocks of V
+    struct Raw {
+        u32x4 k[KC], v[DW];
+        float k_scale, v_scale;
+        bool bad;
+    };
+    auto pages_of = [&](int t0, int32_t &pk, int32_t &pv) {
+        pk = table[min((t0 + (col / 4) * 16) >> g.c.page_shift, last_page)];
+        pv = table[min((t0 + grp * 16) >> g.c.page_shift, last_page)];
+    };
+    auto fetch = [&](Raw &t, int t0, int32_t pk, int32_t pv) {
+        t.bad = pv < 0 || pv >= g.c.pages;
+        if (t.bad) raise_error(g.c);
+        pk = pk < 0 || pk >= g.c.pages ? 0 : pk;
+        pv = t.bad ? 0 : pv;
+        const int64_t bk = static_cast<int64_t>(pk) * g.c.kv_heads + p.kv, bv = static_cast<int64_t>(pv) * g.c.kv_heads + p.kv;
+        const int8_t *k = g.c.k + (bk * size + ((t0 + (col / 4) * 16 + wave * 4 + col % 4) & (size - 1))) * D + grp * 16;
+        const int8_t *v = g.c.v + bv * size * D + ((t0 + grp * 16) & (size - 1)) +
+                          static_cast<int64_t>(wave * DW * 16 + col) * size;
+        t.k_scale = g.c.k_scale[bv];
+        t.v_scale = g.c.v_scale[bv];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dst[e] = static_cast<T>(o[e]);
+        for (int c = 0; c < KC; ++c) t.k[c] = *reinterpret_cast<const u32x4 *>(k + c * 64);
+#pragma unroll
+        for (int d = 0; d < DW; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + static_cast<int64_t>(d) * 16 * size);
+    };
+    // the tile in LDS and what every wavefront knows of it
+    struct Ready {
+        float kc;
+        int step_exp;
+        bool bad;
+    };
+    int step_exp = -200;       // E: log2 of the largest step of V met so far, the same in all wavefronts
+    auto widen_tile = [&](const Raw &t, int buf) {
+        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
+        step_exp = max(step_exp, largest_step(t.v_scale, odd));
+        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
+        const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
+        const h2 vf = {f1, f1}, vbias = {b1, b1};
+        u32x4 *to = frags + buf * kFrags * kWave + lane;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            to[(wave * KH + 2 * c) * kWave] = __builtin_bit_cast(u32x4, widen(t.k[c][0], t.k[c][1]));
+            to[(wave * KH + 2 * c + 1) * kWave] = __builtin_bit_cast(u32x4, widen(t.k[c][2], t.k[c][3]));
+        }
+#pragma unroll
+        for (int d = 0; d < DW; ++d)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+                to[(4 * KH + (wave * DW + d) * 2 + hh) * kWave] =
+                    __builtin_bit_cast(u32x4, widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias));
+        return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, step_exp, t.bad};
+    };
+
+    int my_exp = -200;
+    if (p.begin < p.end) {
+        Raw raw;
+        int32_t pk, pv;
+        pages_of(p.begin, pk, pv);
+        fetch(raw, p.begin, pk, pv);
+        if (p.begin + kTileKeys < p.end) pages_of(p.begin + kTileKeys, pk, pv);
+        Ready ready = widen_tile(raw, 0);
+        int buf = 0;
+        for (int t0 = p.begin; t0 < p.end; t0 += kTileKeys) {
+            const int t1 = t0 + kTileKeys;
+            const bool more = t1 < p.end;
+            if (more) {
+                const int32_t a = pk, b = pv;
+                if (t1 + kTileKeys < p.end) pages_of(t1 + kTileKeys, pk, pv);
+                fetch(raw, t1, a, b);
             }
-        } else {
-            *reinterpret_cast<f32x4 *>(g.part + (split * all_rows + at) * D + d) = o;
-            if (d == 0)
-                reinterpret_cast<float2 *>(g.part + g.splits * all_rows * D)[split * all_rows + at] = float2{top, total};
+            __syncthreads();      // this tile is in LDS, and the other buffer has been read by everyone
+            if (t0 < my_end) {
+                if (ready.step_exp > my_exp) {
+                    soft.rescale(ldexpf(1.f, my_exp - ready.step_exp));
+                    my_exp = ready.step_exp;
+                }
+                const u32x4 *from = frags + buf * kFrags * kWave + lane;
+                soft.tile(
+                    rows, [&](int j, int q) { return __builtin_bit_cast(h8, from[(j * KH + q) * kWave]); },
+                    [&](int d, int hh) { return __builtin_bit_cast(h8, from[(4 * KH + d * 2 + hh) * kWave]); }, ready.kc,
+                    t0, t1 > my_least || __any(ready.bad), ready.bad);
+            }
+            buf ^= 1;
+            if (more) ready = widen_tile(raw, buf);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float total = across_groups_sum(soft.sum[n]);
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const int r = my_r0 + n * 16 + col;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            f32x4 o = soft.acc[d][n] * inv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], my_exp);
+            put_output<T, D>(g, p.s, p.kv, r, p.split, d * 16 + grp * 4, o, soft.ref[n], total);
         }
     }
 }
@@ -430,27 +638,29 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
 
 // How a call is cut: rows per block, tiles of rows, splits of the keys.
 struct Plan {
+    bool many;
     int nt;
     int64_t pieces;
     int32_t splits, chunk;
     bool one_each;
     size_t workspace;
 };
-constexpr int kWaves = 4;
+constexpr int kFewWaves = 4;
 
 Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
     Plan p{};
     const int64_t rep = heads / c.kv_heads, rows = c.max_new * rep;
-    p.nt = rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
-    const int64_t tile = 16 * p.nt;
+    p.many = rows > 32;
+    p.nt = p.many ? (head_dim == 64 ? 4 : 2) : rows <= 16 || head_dim == 128 ? 1 : 2;
+    const int64_t tile = 16 * p.nt * (p.many ? kManyWaves : 1);
     p.one_each = rows <= tile;
     p.pieces = p.one_each ? c.seqs : c.rows * rep / tile + c.seqs;
-    const int64_t step = kTileKeys * kWaves;
+    const int64_t step = kTileKeys * (p.many ? 1 : kFewWaves);
     const int64_t len = c.max_length > 0 ? c.max_length : 1;
     const int64_t blocks = p.pieces * c.kv_heads;
     int64_t splits = (2 * kNumCU + blocks - 1) / blocks;
-    if (p.nt == 1 && splits < (len + 4095) / 4096) splits = (len + 4095) / 4096;
-    const int64_t most = (len + step - 1) / step;
+    if (!p.many && splits < (len + 4095) / 4096) splits = (len + 4095) / 4096;
+    const int64_t most = p.many ? (len + 511) / 512 : (len + step - 1) / step;
     splits = splits < most ? splits : most;
     splits = splits < 64 ? splits : 64;
     const int64_t chunk = ((len + splits - 1) / splits + step - 1) / step * step;
@@ -461,12 +671,18 @@ Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
 }
 
 template <typename T, int D, int NT>
-int32_t launch_attend(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
-    constexpr int lds = kWaves * 16 * NT * ((D + 4) * 4 + 8);
-    auto kern = attend_kernel<T, D, NT, kWaves>;
-    static DynamicLdsGrant grant;
-    if (const int32_t bad = grant.ensure(kern, lds); bad != RMLK_OK) return bad;
-    kern<<<static_cast<uint32_t>(blocks), kWaves * kWave, lds, st>>>(g);
+int32_t launch_few(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
+    constexpr int lds = kFewWaves * 16 * NT * ((D + 4) * 4 + 8);
+    attend_few_kernel<T, D, NT, kFewWaves><<<static_cast<uint32_t>(blocks), kFewWaves * kWave, lds, st>>>(g);
+    return launch_status();
+}
+
+template <typename T, int D>
+int32_t launch_many(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
+    constexpr int NT = D == 64 ? 4 : 2;
+    constexpr int lds = 2 * (4 * (D / 32) + 2 * (D / 16)) * kWave * 16;
+    static_assert(lds <= 64 * 1024, "no more than a block has without asking");
+    attend_many_kernel<T, D, NT><<<static_cast<uint32_t>(blocks), kManyWaves * kWave, lds, st>>>(g);
     return launch_status();
 }
 
@@ -533,13 +749,9 @@ int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk
         g.chunk = plan.chunk;
         g.one_each = plan.one_each;
         int32_t bad;
-        if (d == 64) {
-            bad = plan.nt == 1   ? launch_attend<T, 64, 1>(st, g, blocks)
-                  : plan.nt == 2 ? launch_attend<T, 64, 2>(st, g, blocks)
-                                 : launch_attend<T, 64, 4>(st, g, blocks);
-        } else {
-            bad = plan.nt == 1 ? launch_attend<T, 128, 1>(st, g, blocks) : launch_attend<T, 128, 2>(st, g, blocks);
-        }
+        if (plan.many) bad = d == 64 ? launch_many<T, 64>(st, g, blocks) : launch_many<T, 128>(st, g, blocks);
+        else if (d == 64) bad = plan.nt == 1 ? launch_few<T, 64, 1>(st, g, blocks) : launch_few<T, 64, 2>(st, g, blocks);
+        else bad = launch_few<T, 128, 1>(st, g, blocks);
         if (bad != RMLK_OK || plan.splits == 1) return bad;
         if (d == 64) attend_join_kernel<T, 64><<<static_cast<uint32_t>(join_blocks), 256, 0, st>>>(g);
         else attend_join_kernel<T, 128><<<static_cast<uint32_t>(join_blocks), 256, 0, st>>>(g);
