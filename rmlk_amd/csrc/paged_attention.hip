@@ -51,6 +51,7 @@ struct AttendArgs {
     float scale;         // of the scores, with log2(e)
     int32_t pieces;      // row tiles the grid covers, per KV head and split
     int32_t splits, chunk;   // tokens per split, a multiple of the tile
+    int32_t fold;        // the second half of the tiles in ascending order
     int32_t one_each;    // a sequence has at most one row tile: tile number = sequence
 };
 
@@ -322,7 +323,10 @@ __device__ __forceinline__ bool find_place(const AttendArgs<T> &g, int tile_rows
     p.kv = blockIdx.x % g.c.kv_heads;
     const int rest = blockIdx.x / g.c.kv_heads;
     p.split = rest % g.splits;
-    const int piece = g.pieces - 1 - rest / g.splits;
+    // (in a launch that fits the chip at once the second half goes the other way: the blocks that share a compute
+    // unit then have the same work together)
+    const int order = rest / g.splits, half = (g.pieces + 1) / 2;
+    const int piece = !g.fold || order < half ? g.pieces - 1 - order : order - half;
     if (!locate(g.c, [&](int32_t first, int i) { return (g.one_each ? 0 : first * g.rep / tile_rows) + i <= piece; }, p.seq,
                 p.s)) {
         if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(g.c);
@@ -603,37 +607,56 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     }
 }
 
-// The splits of the rows that see more than one: a wavefront per (row, head).
+// The splits of the rows that see more than one, joined: D / 4 lanes per (row, head).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
-    const int lane = threadIdx.x % kWave;
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
     const int64_t all_rows = g.c.rows * g.heads;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    const int64_t row = at / g.heads;
+    const int64_t at0 = static_cast<int64_t>(blockIdx.x) * kRows, at = at0 + threadIdx.x / kLanes;
+    const int64_t row0 = at0 / g.heads, row = at / g.heads;
+    const int d = threadIdx.x % kLanes * 4;
     int seq;
     Sequence s;
-    if (!locate(g.c, [&](int32_t first, int) { return first <= row; }, seq, s) || at >= all_rows || seq < 0 ||
-        !in_bounds(g.c, s) || row >= s.row + s.fresh)
+    if (!locate(g.c, [&](int32_t first, int) { return first <= row0; }, seq, s) || at >= all_rows) return;
+    if (seq < 0 || row >= s.row + s.fresh) {      // (not the sequence of the block's first row)
+        if (!sequence_of_row(g.c, row, s)) return;
+    } else if (!in_bounds(g.c, s)) {
         return;
+    }
     const int limit = s.length - s.fresh + static_cast<int>(row - s.row) + 1;
     if (limit <= g.chunk) return;
     const int parts = (limit + g.chunk - 1) / g.chunk;
     const float2 *stats = reinterpret_cast<const float2 *>(g.part + g.splits * all_rows * D) + at;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += kWave) top = fmaxf(top, stats[i * all_rows].x);
-    top = wave_max(top);
-    constexpr int N = D / kWave;
-    float o[N] = {}, total = 0.f;
-    for (int i = 0; i < parts; ++i) {
-        const float2 st = stats[i * all_rows];
-        const float weight = st.y == 0.f ? 0.f : st.y * __builtin_amdgcn_exp2f(st.x - top);
-        total += weight;
+    const float *part = g.part + at * D + d;
+    // groups of eight parts, their loads in flight together; the reference point moves between groups
+    constexpr int kGroup = 8;
+    float top = -INFINITY, total = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < parts; i0 += kGroup) {
+        float2 st[kGroup];
+        f32x4 v[kGroup];
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = fmaf(g.part[(i * all_rows + at) * D + lane * N + e], weight, o[e]);
+        for (int i = 0; i < kGroup; ++i) {
+            const int64_t from = min(i0 + i, parts - 1) * all_rows;
+            st[i] = stats[from];
+            v[i] = *reinterpret_cast<const f32x4 *>(part + from * D);
+            if (i0 + i >= parts) st[i].y = 0.f;
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) now = fmaxf(now, st[i].x);
+        const float alpha = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - now);
+        top = now;
+        total *= alpha;
+        o *= alpha;
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+            const float weight = st[i].y == 0.f ? 0.f : st[i].y * __builtin_amdgcn_exp2f(st[i].x - top);
+            total += weight;
+            o += v[i] * weight;
+        }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int e = 0; e < N; ++e) g.out[at * D + lane * N + e] = static_cast<T>(o[e] * inv);
+    store_four(g.out + at * D + d, o * (total == 0.f ? 0.f : 1.f / total));
 }
 
 // How a call is cut: rows per block, tiles of rows, splits of the keys.
@@ -651,16 +674,22 @@ Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
     Plan p{};
     const int64_t rep = heads / c.kv_heads, rows = c.max_new * rep;
     p.many = rows > 32;
-    p.nt = p.many ? (head_dim == 64 ? 4 : 2) : rows <= 16 || head_dim == 128 ? 1 : 2;
+    p.nt = p.many ? 2 : rows <= 16 || head_dim == 128 ? 1 : 2;
     const int64_t tile = 16 * p.nt * (p.many ? kManyWaves : 1);
     p.one_each = rows <= tile;
     p.pieces = p.one_each ? c.seqs : c.rows * rep / tile + c.seqs;
     const int64_t step = kTileKeys * (p.many ? 1 : kFewWaves);
     const int64_t len = c.max_length > 0 ? c.max_length : 1;
     const int64_t blocks = p.pieces * c.kv_heads;
-    int64_t splits = (2 * kNumCU + blocks - 1) / blocks;
+    // Splits: enough blocks for every compute unit to have some at a time, and for rows behind a long cache
+    // pieces short enough to even out sequences of different lengths; not for prompts that fill the chip by
+    // themselves (a part costs its rows a trip through memory and the call a second kernel).
+    int64_t splits;
+    if (p.many) splits = (c.max_length > 2 * c.max_new ? 6 : 3) * kNumCU / blocks;
+    else splits = (2 * kNumCU + blocks - 1) / blocks;
     if (!p.many && splits < (len + 4095) / 4096) splits = (len + 4095) / 4096;
-    const int64_t most = p.many ? (len + 511) / 512 : (len + step - 1) / step;
+    if (splits < 1) splits = 1;
+    const int64_t most = p.many ? (len + 1023) / 1024 : (len + step - 1) / step;
     splits = splits < most ? splits : most;
     splits = splits < 64 ? splits : 64;
     const int64_t chunk = ((len + splits - 1) / splits + step - 1) / step * step;
@@ -679,7 +708,7 @@ int32_t launch_few(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
 
 template <typename T, int D>
 int32_t launch_many(hipStream_t st, const AttendArgs<T> &g, int64_t blocks) {
-    constexpr int NT = D == 64 ? 4 : 2;
+    constexpr int NT = 2;
     constexpr int lds = 2 * (4 * (D / 32) + 2 * (D / 16)) * kWave * 16;
     static_assert(lds <= 64 * 1024, "no more than a block has without asking");
     attend_many_kernel<T, D, NT><<<static_cast<uint32_t>(blocks), kManyWaves * kWave, lds, st>>>(g);
@@ -726,7 +755,7 @@ int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk
     if (q_stride % unit || !aligned16(q) || !aligned16(out)) return RMLK_ERR_UNSUPPORTED;
     const Plan plan = plan_for(c, dtype, d, heads);
     const int64_t blocks = plan.pieces * c.kv_heads * plan.splits;
-    const int64_t join_blocks = (c.rows * heads + 3) / 4;
+    const int64_t join_blocks = (c.rows * heads * (d / 4) + 255) / 256;
     if (blocks > (1 << 23) || join_blocks > (1 << 23) || c.rows * heads > 0x3fffffff) return RMLK_ERR_TOO_LARGE;
     if (plan.workspace > 0) {
         if (!workspace) return RMLK_ERR_NULL_POINTER;
@@ -748,6 +777,7 @@ int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk
         g.splits = plan.splits;
         g.chunk = plan.chunk;
         g.one_each = plan.one_each;
+        g.fold = plan.many && blocks <= 3 * kNumCU;
         int32_t bad;
         if (plan.many) bad = d == 64 ? launch_many<T, 64>(st, g, blocks) : launch_many<T, 128>(st, g, blocks);
         else if (d == 64) bad = plan.nt == 1 ? launch_few<T, 64, 1>(st, g, blocks) : launch_few<T, 64, 2>(st, g, blocks);
