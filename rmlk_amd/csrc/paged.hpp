@@ -120,34 +120,90 @@ __device__ __forceinline__ bool in_bounds(const PagedArgs &g, const Sequence &q)
     return q.fresh <= g.max_new && q.length >= 0 && q.length <= g.max_length;
 }
 
-// One trip over `first` and `length` by every wavefront for itself (a few cache lines): false when `first`
-// does not ascend within 0 .. rows; otherwise the last sequence s with begins(first[s], s), which has to hold
-// for a run of sequences from 0 on, and its numbers (s = -1: none). The work of a ragged call is numbered
-// so that sequence s has the numbers from first[s] / unit + extra * s on, floor(its rows / unit) + extra of
-// them at least: a grid of rows / unit + extra * seqs blocks covers every sequence without a rectangle over
-// the longest one.
-template <typename F>
-__device__ __forceinline__ bool locate(const PagedArgs &g, F &&begins, int &s, Sequence &q) {
-    s = -1;
+// The work of a ragged call, cut into items: sequence s has count(its numbers) of them, numbered one after
+// the other, so that the grid (an upper bound of their sum) has its idle blocks at the end only: idle
+// blocks among the others leave compute units with less work than their neighbours. Every wavefront
+// works the numbering out for itself in one trip over `first` and `length` (a few cache lines).
+struct Item {
+    int s;            // its sequence, -1: none (the number is behind the last item)
+    int index;        // among the sequence's items
+    Sequence q;
+};
+struct NoOrder {
+    __device__ __forceinline__ int operator()(int, int item) const { return item; }
+};
+
+__device__ __forceinline__ int wave_prefix_sum(int v) {
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) {
+        const int from = __shfl_up(v, step, kWave);
+        v += static_cast<int>(threadIdx.x % kWave) >= step ? from : 0;
+    }
+    return v;
+}
+
+// Item number order(total, item). False when `first` does not ascend within 0 .. rows; a sequence that leaves
+// the call's bounds counts as one item (which reports it).
+template <typename C, typename O = NoOrder>
+__device__ __forceinline__ bool find_item(const PagedArgs &g, int item, C &&count, Item &found, O &&order = O{}) {
+    const int lane = static_cast<int>(threadIdx.x % kWave);
+    auto numbers = [&](int i, Sequence &q, bool &good) {
+        q.row = g.first[i];
+        q.fresh = g.first[i + 1] - q.row;
+        q.length = g.length[i];
+        good = good && q.row >= 0 && q.fresh >= 0 && q.row + static_cast<int64_t>(q.fresh) <= g.rows;
+        return q.fresh == 0 ? 0 : in_bounds(g, q) ? count(q) : 1;
+    };
+    found.s = -1;
     bool good = true;
+    if (g.seqs == 1) {
+        const int n = numbers(0, found.q, good);
+        if (!good) return false;
+        item = order(n, item);
+        if (item >= 0 && item < n) {
+            found.s = 0;
+            found.index = item;
+        }
+        return true;
+    }
+    int total = 0;
+    if (g.seqs > kWave) {
+        for (int base = 0; base < g.seqs; base += kWave) {
+            Sequence q;
+            int n = 0;
+            if (base + lane < g.seqs) n = numbers(base + lane, q, good);
+            total += __builtin_amdgcn_readlane(wave_prefix_sum(n), kWave - 1);
+        }
+        item = order(total, item);
+    }
+    int before = 0;
     for (int base = 0; base < g.seqs; base += kWave) {
-        const int i = base + static_cast<int>(threadIdx.x % kWave);
-        int32_t lo = 0, hi = 0, length = 0;
-        bool before = false;
-        if (i < g.seqs) {
-            lo = g.first[i];
-            hi = g.first[i + 1];
-            length = g.length[i];
-            good = good && lo >= 0 && lo <= hi && hi <= g.rows;
-            before = begins(lo, i);
+        Sequence q{0, 0, 0};
+        int n = 0;
+        if (base + lane < g.seqs) n = numbers(base + lane, q, good);
+        const int upto = before + wave_prefix_sum(n);
+        const int last = __builtin_amdgcn_readlane(upto, kWave - 1);
+        if (g.seqs <= kWave) item = order(last, item);
+        const uint64_t here = __ballot(item >= upto - n && item < upto);
+        if (here) {
+            const int at = __ffsll(static_cast<unsigned long long>(here)) - 1;
+            found.s = base + at;
+            found.index = item - __builtin_amdgcn_readlane(upto - n, at);
+            found.q.row = __builtin_amdgcn_readlane(q.row, at);
+            found.q.fresh = __builtin_amdgcn_readlane(q.fresh, at);
+            found.q.length = __builtin_amdgcn_readlane(q.length, at);
         }
-        const int n = __popcll(__ballot(before));
-        if (n > 0) {
-            s = base + n - 1;
-            q.row = __builtin_amdgcn_readlane(lo, n - 1);
-            q.fresh = __builtin_amdgcn_readlane(hi, n - 1) - q.row;
-            q.length = __builtin_amdgcn_readlane(length, n - 1);
-        }
+        before = last;
+    }
+    return __all(good);
+}
+
+// first[0 .. seqs] ascends within 0 .. rows.
+__device__ __forceinline__ bool starts_ascend(const PagedArgs &g) {
+    bool good = true;
+    for (int i = static_cast<int>(threadIdx.x % kWave); i < g.seqs; i += kWave) {
+        const int32_t lo = g.first[i], hi = g.first[i + 1];
+        good = good && lo >= 0 && lo <= hi && hi <= g.rows;
     }
     return __all(good);
 }

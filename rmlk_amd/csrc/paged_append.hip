@@ -25,7 +25,7 @@ struct AppendArgs {
     int64_t k_stride, v_stride, q_stride;
     int64_t positions;
     int32_t heads;
-    int32_t pieces;      // upper bound of (sequence, page) pairs: the first blocks of the grid, per KV head
+    int32_t pieces;      // upper bound of the pages written to: the first blocks of the grid, per KV head
     int64_t q_units;     // units of q: D / 16 per row and kHeads heads
 };
 
@@ -104,14 +104,8 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
     __shared__ __align__(16) uint8_t turned[D][kPad];
     const int tid = threadIdx.x, lane = tid % kWave;
     const int kv_blocks = g.pieces * g.c.kv_heads;
-    const int piece = blockIdx.x / g.c.kv_heads, head = blockIdx.x % g.c.kv_heads;
-    int s;
-    Sequence q;
-    if (!locate(g.c, [&](int32_t first, int i) { return (first >> g.c.page_shift) + 2 * i <= piece; }, s, q)) {
-        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
-        return;
-    }
     if (static_cast<int>(blockIdx.x) >= kv_blocks) {
+        if (!starts_ascend(g.c)) return;
         const int64_t first_unit = (static_cast<int64_t>(blockIdx.x) - kv_blocks) * THREADS;
         // a unit: eight + eight dims of kHeads heads of a row, which share their row of the tables
         const int groups = (g.heads + kHeads - 1) / kHeads;
@@ -119,6 +113,7 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
             const int64_t rg = u / kUnitsK;
             const int d = static_cast<int>(u % kUnitsK) * 8;
             const int row = static_cast<int>(rg / groups), h0 = static_cast<int>(rg % groups) * kHeads;
+            Sequence q;
             if (!sequence_of_row(g.c, row, q) || q.length < q.fresh) continue;
             const int64_t pos = q.length - q.fresh + (row - q.row);
             if (g.cos && pos >= g.positions) continue;
@@ -144,17 +139,29 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
         }
         return;
     }
-    if (s < 0) return;
-    const int index = piece - ((q.row >> g.c.page_shift) + 2 * s);   // of the pages it writes to
+    const int head = blockIdx.x % g.c.kv_heads;
+    Item item;
+    // (a sequence's items: the pages it writes to)
+    if (!find_item(g.c, blockIdx.x / g.c.kv_heads,
+                   [&](const Sequence &q) {
+                       const int last = (q.length - 1) >> g.c.page_shift, begin = (q.length - q.fresh) >> g.c.page_shift;
+                       return q.length < q.fresh ? 1 : last - begin + 1;
+                   },
+                   item)) {
+        if (blockIdx.x == 0 && tid == 0) raise_error(g.c);
+        return;
+    }
+    if (item.s < 0) return;
+    const Sequence q = item.q;
+    const int s = item.s, index = item.index;
     if (!in_bounds(g.c, q) || q.length < q.fresh) {
-        if (index == 0 && head == 0 && tid == 0) raise_error(g.c);
+        if (head == 0 && tid == 0) raise_error(g.c);
         return;
     }
     const int size = 1 << g.c.page_shift;
     const int begin_pos = q.length - q.fresh;
     const int64_t page_at = static_cast<int64_t>(begin_pos >> g.c.page_shift) + index;   // in the table
     const int64_t page_pos = page_at << g.c.page_shift;
-    if (index < 0 || q.fresh == 0 || page_pos >= q.length) return;
     const int slot0 = page_pos < begin_pos ? static_cast<int>(begin_pos - page_pos) : 0;
     int slot1 = static_cast<int>(min(static_cast<int64_t>(size), q.length - page_pos));
     const int32_t page = g.c.table[s * g.c.table_stride + page_at];

@@ -49,10 +49,8 @@ struct AttendArgs {
     int64_t q_stride;
     int32_t heads, rep;
     float scale;         // of the scores, with log2(e)
-    int32_t pieces;      // row tiles the grid covers, per KV head and split
     int32_t splits, chunk;   // tokens per split, a multiple of the tile
-    int32_t fold;        // the second half of the tiles in ascending order
-    int32_t one_each;    // a sequence has at most one row tile: tile number = sequence
+    int32_t fold;        // the second half of the items in ascending order
 };
 
 // the four bytes of a word as halves 1024 + (b + 128)
@@ -195,71 +193,75 @@ struct Softmax {
 #pragma unroll
             for (int n = 0; n < NT; ++n) c[n] = rows.limit[n] <= t0 + grp * 16 || bad ? kLeastFactor : c[n];
         }
+        f32x4 sc[4][NT];
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            f32x4 sc[2][NT];
+        for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int n = 0; n < NT; ++n) sc[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) sc[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int q = 0; q < KH; ++q) {
+                const h8 kf = k_frag(j, q);
 #pragma unroll
-                for (int q = 0; q < KH; ++q) {
-                    const h8 kf = k_frag(2 * hh + j, q);
+                for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-                    for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, rows.q[p][n][q], sc[j][n], 0, 0, 0);
-                }
+                    for (int n = 0; n < NT; ++n)
+                        sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, rows.q[p][n][q], sc[j][n], 0, 0, 0);
             }
-            if (masked) {
-                const int key = t0 + grp * 16 + hh * 8;
+        }
+        if (masked) {
+            const int key = t0 + grp * 16;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        sc[i / 4][n][i % 4] = key + i < rows.limit[n] && !bad ? sc[i / 4][n][i % 4] : -INFINITY;
-            }
-            // exponents relative to the reference point (which is finite: a hidden score stays -inf)
-            auto exponent = [&](int n, int i) { return fmaf(sc[i / 4][n][i % 4], c[n], -ref[n]); };
-            bool beyond = false;
+                for (int i = 0; i < 16; ++i)
+                    sc[i / 4][n][i % 4] = key + i < rows.limit[n] && !bad ? sc[i / 4][n][i % 4] : -INFINITY;
+        }
+        // exponents relative to the reference point (which is finite: a hidden score stays -inf)
+        auto exponent = [&](int n, int i) { return fmaf(sc[i / 4][n][i % 4], c[n], -ref[n]); };
+        bool beyond = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, exponent(n, i));
+            beyond = top > kMostWeight || beyond;
+        }
+        if (__any(beyond)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, exponent(n, i));
-                beyond = top > kMostWeight || beyond;
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i / 4][n][i % 4] * c[n]);
+                const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
+                const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
+                ref[n] = now;
+                sum[n] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
             }
-            if (__any(beyond)) {
+        }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[i / 4][n][i % 4] * c[n]);
-                    const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
-                    const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
-                    ref[n] = now;
-                    sum[n] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
-                }
-            }
+        for (int hh = 0; hh < 2; ++hh) {
             h8 pf[P][NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                    const f32x2 w = {__builtin_amdgcn_exp2f(exponent(n, i)), __builtin_amdgcn_exp2f(exponent(n, i + 1))};
-                    sum[n] += w[0];
-                    sum[n] += w[1];
+                    const f32x2 w = {__builtin_amdgcn_exp2f(exponent(n, hh * 8 + i)),
+                                     __builtin_amdgcn_exp2f(exponent(n, hh * 8 + i + 1))};
                     const h2 hi = __builtin_convertvector(w, h2);
                     pf[0][n][i] = hi[0];
                     pf[0][n][i + 1] = hi[1];
                     if constexpr (P == 2) {
+                        sum[n] += w[0];
+                        sum[n] += w[1];
                         const f32x2 rest = {w[0] - static_cast<float>(hi[0]), w[1] - static_cast<float>(hi[1])};
                         const h2 lo = __builtin_convertvector(rest, h2);
                         pf[1][n][i] = lo[0];
                         pf[1][n][i + 1] = lo[1];
+                    } else {
+                        // (the sum of the weights as they are multiplied: their rounding cancels in part)
+                        sum[n] = __builtin_amdgcn_fdot2(hi, h2{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, sum[n], false);
                     }
                 }
 #pragma unroll
@@ -318,29 +320,34 @@ struct Place {
 template <typename T>
 __device__ __forceinline__ bool find_place(const AttendArgs<T> &g, int tile_rows, Place &p) {
     // Blocks of one KV head next to each other would meet on different XCDs (workgroups go round robin): the
-    // head is the fastest index, so with eight of them an XCD reads one head's cache. Last row tiles first:
-    // they see the most keys.
+    // head is the fastest index, so with eight of them an XCD reads one head's cache.
     p.kv = blockIdx.x % g.c.kv_heads;
-    const int rest = blockIdx.x / g.c.kv_heads;
-    p.split = rest % g.splits;
-    // (in a launch that fits the chip at once the second half goes the other way: the blocks that share a compute
-    // unit then have the same work together)
-    const int order = rest / g.splits, half = (g.pieces + 1) / 2;
-    const int piece = !g.fold || order < half ? g.pieces - 1 - order : order - half;
-    if (!locate(g.c, [&](int32_t first, int i) { return (g.one_each ? 0 : first * g.rep / tile_rows) + i <= piece; }, p.seq,
-                p.s)) {
+    // A sequence's items: its row tiles for every split it reaches. Last items first: with a causal prompt they
+    // see the most keys; in a launch that fits the chip at once (fold) the second half of them goes the other
+    // way, so that the blocks that share a compute unit have the same work together.
+    auto tiles = [&](const Sequence &q) { return (q.fresh * g.rep + tile_rows - 1) / tile_rows; };
+    Item item;
+    if (!find_item(g.c, blockIdx.x / g.c.kv_heads,
+                   [&](const Sequence &q) { return tiles(q) * (q.length <= g.chunk ? 1 : (q.length + g.chunk - 1) / g.chunk); },
+                   item,
+                   [&](int total, int order) {
+                       const int half = (total + 1) / 2;
+                       return order >= total ? -1 : !g.fold || order < half ? total - 1 - order : order - half;
+                   })) {
         if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(g.c);
         return false;
     }
-    if (p.seq < 0) return false;
+    if (item.s < 0) return false;
+    p.s = item.q;
+    p.seq = item.s;
     if (!in_bounds(g.c, p.s)) {
         if (threadIdx.x == 0) raise_error(g.c);
         return false;
     }
-    const int index = g.one_each ? 0 : piece - (p.s.row * g.rep / tile_rows + p.seq);
+    const int row_tiles = tiles(p.s);
+    p.split = item.index / row_tiles;
     p.rows = p.s.fresh * g.rep;
-    p.r0 = index * tile_rows;
-    if (index < 0 || p.r0 >= p.rows) return false;
+    p.r0 = (item.index - p.split * row_tiles) * tile_rows;
     const int past = p.s.length - p.s.fresh;           // position of the sequence's first row
     p.most = past + min(p.r0 + tile_rows - 1, p.rows - 1) / g.rep + 1;   // tokens the last row sees
     p.least = past + p.r0 / g.rep + 1;
@@ -612,17 +619,11 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
     constexpr int kLanes = D / 4, kRows = 256 / kLanes;
     const int64_t all_rows = g.c.rows * g.heads;
-    const int64_t at0 = static_cast<int64_t>(blockIdx.x) * kRows, at = at0 + threadIdx.x / kLanes;
-    const int64_t row0 = at0 / g.heads, row = at / g.heads;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+    const int64_t row = at / g.heads;
     const int d = threadIdx.x % kLanes * 4;
-    int seq;
     Sequence s;
-    if (!locate(g.c, [&](int32_t first, int) { return first <= row0; }, seq, s) || at >= all_rows) return;
-    if (seq < 0 || row >= s.row + s.fresh) {      // (not the sequence of the block's first row)
-        if (!sequence_of_row(g.c, row, s)) return;
-    } else if (!in_bounds(g.c, s)) {
-        return;
-    }
+    if (!starts_ascend(g.c) || at >= all_rows || !sequence_of_row(g.c, row, s)) return;
     const int limit = s.length - s.fresh + static_cast<int>(row - s.row) + 1;
     if (limit <= g.chunk) return;
     const int parts = (limit + g.chunk - 1) / g.chunk;
@@ -665,7 +666,6 @@ struct Plan {
     int nt;
     int64_t pieces;
     int32_t splits, chunk;
-    bool one_each;
     size_t workspace;
 };
 constexpr int kFewWaves = 4;
@@ -676,20 +676,31 @@ Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
     p.many = rows > 32;
     p.nt = p.many ? 2 : rows <= 16 || head_dim == 128 ? 1 : 2;
     const int64_t tile = 16 * p.nt * (p.many ? kManyWaves : 1);
-    p.one_each = rows <= tile;
-    p.pieces = p.one_each ? c.seqs : c.rows * rep / tile + c.seqs;
+    // upper bound of the row tiles; exact where all sequences bring the same rows
+    const int64_t ragged = c.rows * rep / tile + c.seqs, even = c.seqs * ((rows + tile - 1) / tile);
+    p.pieces = ragged < even ? ragged : even;
     const int64_t step = kTileKeys * (p.many ? 1 : kFewWaves);
     const int64_t len = c.max_length > 0 ? c.max_length : 1;
     const int64_t blocks = p.pieces * c.kv_heads;
-    // Splits: enough blocks for every compute unit to have some at a time, and for rows behind a long cache
-    // pieces short enough to even out sequences of different lengths; not for prompts that fill the chip by
-    // themselves (a part costs its rows a trip through memory and the call a second kernel).
+    // Splits of the keys. A part costs its rows a trip through memory, and the call a second kernel.
+    // Many rows: as many as make two blocks per compute unit (they are resident together: 512 rows behind 8192
+    // keys, 8 KV heads of 128 dims, take 103 us in 4 splits = 512 blocks, 115 us in 8); in a ragged call, where
+    // most sequences do not reach the bounds, four times that (the six sequences of the benchmark: 142 us,
+    // 182 us with the former rule); prompts with little before them are not thinned out for being ragged.
+    // Few rows: a block per compute unit, and pieces of 2048 keys beyond 4096, so that sequences of different
+    // lengths even out (64 sequences of 100 .. 16384 keys: 91 us, in pieces of 4096 109 us, of 1024 97 us; 32
+    // sequences of 4096 keys: 52 us in one piece, 57 us in two). Up to 1024 keys the second kernel costs more
+    // than it saves.
     int64_t splits;
-    if (p.many) splits = (c.max_length > 2 * c.max_new ? 6 : 3) * kNumCU / blocks;
-    else splits = (2 * kNumCU + blocks - 1) / blocks;
-    if (!p.many && splits < (len + 4095) / 4096) splits = (len + 4095) / 4096;
+    if (p.many) {
+        const bool uneven = c.rows < c.seqs * c.max_new && c.max_length > 2 * c.max_new;
+        splits = (uneven ? 8 : 2) * kNumCU / blocks;
+    } else {
+        splits = len <= 1024 ? 1 : (kNumCU + blocks - 1) / blocks;
+        if (len > 4096 && splits < (len + 2047) / 2048) splits = (len + 2047) / 2048;
+    }
     if (splits < 1) splits = 1;
-    const int64_t most = p.many ? (len + 1023) / 1024 : (len + step - 1) / step;
+    const int64_t most = p.many ? (len + 511) / 512 : (len + step - 1) / step;
     splits = splits < most ? splits : most;
     splits = splits < 64 ? splits : 64;
     const int64_t chunk = ((len + splits - 1) / splits + step - 1) / step * step;
@@ -773,10 +784,8 @@ int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk
         g.heads = static_cast<int32_t>(heads);
         g.rep = static_cast<int32_t>(heads / c.kv_heads);
         g.scale = (scale_is_mul ? scale : 1.f / scale) * kLog2e;
-        g.pieces = static_cast<int32_t>(plan.pieces);
         g.splits = plan.splits;
         g.chunk = plan.chunk;
-        g.one_each = plan.one_each;
         g.fold = plan.many && blocks <= 3 * kNumCU;
         int32_t bad;
         if (plan.many) bad = d == 64 ? launch_many<T, 64>(st, g, blocks) : launch_many<T, 128>(st, g, blocks);
