@@ -517,47 +517,69 @@ def gemv_kmajor_head_rows(x, wt, k: int, streams, first_cols, gamma=None, eps: f
 
 # ---- 8-bit serving: int8 rows and products, a paged int8 cache ----------------------------------------
 
-def _rows(t, width: int) -> int:
+def _pitch(t, width: int) -> int:
     """Elements from one row to the next of a tensor [rows, ...] whose rows hold `width` dense elements."""
     dense = 1
     for d in range(t.dim() - 1, 0, -1):
-        assert t.shape[d] == 1 or t.stride(d) == dense, "the elements of a row must be dense"
-        dense *= t.shape[d]
+        n = t.shape[d]
+        assert n == 1 or t.stride(d) == dense, "the elements of a row must be dense"
+        dense *= n
     assert dense == width, f"rows hold {dense} elements, {width} expected"
-    _here(t)
     return max(t.stride(0), width) if t.shape[0] > 1 else width
 
 
-def _here(*tensors) -> None:
-    """The launch goes to the current stream of the current device: its operands have to lie there."""
+def _pitch2(t) -> int:
+    """The same for a matrix."""
+    rows, cols = t.shape
+    pitch, one = t.stride()
+    assert one == 1 or cols == 1, "the elements of a row must be dense"
+    return pitch if rows > 1 and pitch > cols else cols
+
+
+def _raw_stream(*tensors) -> int:
+    """The current stream of the current device, where the operands of a launch have to lie. (The cheap way to
+    ask: a decode step makes these calls one after the other.)"""
+    device = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None:
-            assert t.is_cuda and t.device.index == torch.cuda.current_device(), "tensors must lie on the current device"
+        assert t is None or t.get_device() == device, "tensors must lie on the current device"
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _int8_rows(q, scale, rows: int, cols: int) -> int:
+    assert q.dtype is torch.int8 and scale.dtype is torch.float32 and scale.is_contiguous()
+    assert q.shape[0] == scale.numel() == rows and q.shape[1] >= (cols + 15) // 16 * 16
+    return _pitch2(q)
 
 
 def quantize_rows(x, q, scale) -> None:
     """q int8 [rows, ld] (ld: cols rounded up to 16, or more) and scale float [rows] of x [rows, cols] (float,
     float16 or bfloat16; rows may lie apart): scale = max|row| / 127, q = row / scale to nearest even."""
     rows, cols = x.shape
-    _here(q, scale)
-    assert q.dtype == torch.int8 and q.shape[0] == rows and q.stride(1) == 1 and q.shape[1] >= (cols + 15) // 16 * 16
-    assert scale.dtype == torch.float32 and scale.numel() == rows
-    check(lib().rmlk_hip_quantize_rows(_stream(), storage_of(x), rows, cols, x.data_ptr(), _rows(x, cols),
-                                       q.data_ptr(), _rows(q, q.shape[1]), _ptr(scale)), "rmlk_hip_quantize_rows")
+    stream = _raw_stream(x, q, scale)
+    ldq = _int8_rows(q, scale, rows, cols)
+    status = lib().rmlk_hip_quantize_rows(stream, storage_of(x), rows, cols, x.data_ptr(), _pitch2(x), q.data_ptr(),
+                                          ldq, scale.data_ptr())
+    if status:
+        check(status, "rmlk_hip_quantize_rows")
 
 
 def rmsnorm_quantize_rows(x, gamma, eps: float, q, scale, add=None, sum_out=None) -> None:
     """quantize_rows of x / sqrt(mean(x^2) + eps) * gamma; with `add` of x + add, which also goes to sum_out."""
     rows, cols = x.shape
-    _here(x, gamma, q, scale, add, sum_out)
-    assert q.dtype == torch.int8 and q.shape[0] == rows and q.stride(1) == 1 and q.shape[1] >= (cols + 15) // 16 * 16
-    assert scale.dtype == torch.float32 and scale.numel() == rows
-    assert gamma.dtype == torch.float32 and gamma.numel() == cols
+    stream = _raw_stream(x, gamma, q, scale, add, sum_out)
+    ldq = _int8_rows(q, scale, rows, cols)
+    assert x.is_contiguous() and gamma.dtype is torch.float32 and gamma.shape == (cols,) and gamma.is_contiguous()
     for t in (add, sum_out):
-        assert t is None or (t.dtype == x.dtype and t.shape == x.shape)
-    check(lib().rmlk_hip_rmsnorm_quantize_rows(_stream(), storage_of(x), rows, cols, _ptr(x), _ptr(add), _ptr(gamma),
-                                               float(eps), _ptr(sum_out), q.data_ptr(), _rows(q, q.shape[1]),
-                                               _ptr(scale)), "rmlk_hip_rmsnorm_quantize_rows")
+        assert t is None or (t.dtype is x.dtype and t.shape == x.shape and t.is_contiguous())
+    status = lib().rmlk_hip_rmsnorm_quantize_rows(stream, storage_of(x), rows, cols, x.data_ptr(), _address(add),
+                                                  gamma.data_ptr(), eps, _address(sum_out), q.data_ptr(), ldq,
+                                                  scale.data_ptr())
+    if status:
+        check(status, "rmlk_hip_rmsnorm_quantize_rows")
 
 
 def matmul_int8_workspace_size(m: int, n: int, k: int) -> int:
@@ -568,23 +590,33 @@ def matmul_int8(a, a_scale, wt, w_scale, out, k: int, residual=None, workspace=N
     """out[m, n] = (a[:, :k] . wt[:, :k]^T) * a_scale[:, None] * w_scale[None, :] (+ residual: [m, n], or [n] for
     a bias), a int8 [m, ld] and wt int8 [n, ld] as quantize_rows leaves them."""
     m, n = out.shape
-    _here(a, a_scale, wt, w_scale, residual, workspace)
-    assert a.dtype == wt.dtype == torch.int8 and a.shape[0] == m and wt.shape[0] == n
-    assert 0 <= k <= min(a.shape[1], wt.shape[1])
-    assert a_scale.dtype == w_scale.dtype == torch.float32 and a_scale.numel() == m and w_scale.numel() == n
+    stream = _raw_stream(a, a_scale, wt, w_scale, out, residual, workspace)
+    assert a.dtype is torch.int8 and wt.dtype is torch.int8 and a.shape[0] == m and wt.shape[0] == n
+    assert 0 <= k <= a.shape[1] and k <= wt.shape[1]
+    assert a_scale.dtype is torch.float32 and w_scale.dtype is torch.float32
+    assert a_scale.numel() == m and w_scale.numel() == n and a_scale.is_contiguous() and w_scale.is_contiguous()
     ldr = 0
     if residual is not None:
-        assert residual.dtype == out.dtype and residual.shape in ((m, n), (n,))
-        ldr = _rows(residual, n) if residual.dim() == 2 else 0
-        assert residual.dim() == 2 or residual.is_contiguous()
-    need = matmul_int8_workspace_size(m, n, k)
+        assert residual.dtype is out.dtype
+        if residual.dim() == 2:
+            assert residual.shape == out.shape
+            ldr = _pitch2(residual)
+        else:
+            assert residual.shape == (n,) and residual.is_contiguous()
+    handle = lib()
+    need = handle.rmlk_hip_matmul_int8_workspace_size(m, n, k)
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    check(lib().rmlk_hip_matmul_int8(_stream(), storage_of(out), m, n, k, a.data_ptr(), _rows(a, a.shape[1]),
-                                     _ptr(a_scale), wt.data_ptr(), _rows(wt, wt.shape[1]), _ptr(w_scale),
-                                     residual.data_ptr() if residual is not None else 0, ldr, _ptr(workspace),
-                                     ws_bytes, out.data_ptr(), _rows(out, n)), "rmlk_hip_matmul_int8")
+    ws_bytes = 0
+    if workspace is not None:
+        assert workspace.is_contiguous()
+        ws_bytes = workspace.numel() * workspace.element_size()
+    status = handle.rmlk_hip_matmul_int8(stream, storage_of(out), m, n, k, a.data_ptr(), _pitch2(a),
+                                         a_scale.data_ptr(), wt.data_ptr(), _pitch2(wt), w_scale.data_ptr(),
+                                         _address(residual), ldr, _address(workspace), ws_bytes, out.data_ptr(),
+                                         _pitch2(out))
+    if status:
+        check(status, "rmlk_hip_matmul_int8")
 
 
 class PagedCache:
@@ -631,21 +663,25 @@ def paged_append(cache: PagedCache, batch: PagedBatch, k, v, cos=None, sin=None,
                  err_flag=None) -> None:
     """Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated by row `position` of cos and sin (float
     [positions, head_dim]; None: as it is); q [tokens, heads, head_dim] is rotated alike into q_out."""
-    _here(cache.k, batch.first, cos, sin, q_out, err_flag)
-    width = cache.kv_heads * cache.head_dim
-    assert k.dtype == v.dtype and k.shape[0] == v.shape[0] == batch.tokens
-    heads = 0
+    stream = _raw_stream(cache.k, batch.first, k, v, cos, sin, q, q_out, err_flag)
+    width, positions, heads, q_pitch = cache.kv_heads * cache.head_dim, 0, 0, 0
+    assert k.dtype is v.dtype and k.shape[0] == v.shape[0] == batch.tokens
     if q is not None:
         heads = q.shape[1]
-        assert q.dtype == q_out.dtype == k.dtype and q.shape == q_out.shape == (batch.tokens, heads, cache.head_dim)
-    for t in (cos, sin):
-        assert t is None or (t.dtype == torch.float32 and t.dim() == 2 and t.shape == (cos.shape[0], cache.head_dim))
-    check(lib().rmlk_hip_paged_append(_stream(), storage_of(k), cache.struct, batch.struct, k.data_ptr(),
-                                      _rows(k, width), v.data_ptr(), _rows(v, width), _ptr(cos), _ptr(sin),
-                                      cos.shape[0] if cos is not None else 0, heads,
-                                      q.data_ptr() if q is not None else 0,
-                                      _rows(q, heads * cache.head_dim) if q is not None else 0, _ptr(q_out),
-                                      _ptr(err_flag)), "rmlk_hip_paged_append")
+        assert q.dtype is k.dtype and q_out.dtype is k.dtype and q_out.is_contiguous()
+        assert q.shape == q_out.shape == (batch.tokens, heads, cache.head_dim)
+        q_pitch = _pitch(q, heads * cache.head_dim)
+    if cos is not None:
+        positions = cos.shape[0]
+        assert cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+        assert cos.shape == sin.shape == (positions, cache.head_dim)
+    assert err_flag is None or err_flag.dtype is torch.int32
+    status = lib().rmlk_hip_paged_append(stream, storage_of(k), cache.struct, batch.struct, k.data_ptr(),
+                                         _pitch(k, width), v.data_ptr(), _pitch(v, width), _address(cos),
+                                         _address(sin), positions, heads, _address(q), q_pitch, _address(q_out),
+                                         _address(err_flag))
+    if status:
+        check(status, "rmlk_hip_paged_append")
 
 
 def paged_attention_workspace_size(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype, heads: int) -> int:
@@ -658,16 +694,22 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, scale: float, 
     """out [tokens, heads, head_dim] = causal attention of q over the cached tokens of its sequences; the rows of q
     may lie apart (a slice of a joint projection)."""
     heads = q.shape[1]
-    _here(cache.k, batch.first, out, workspace, err_flag)
-    assert q.dtype == out.dtype and q.shape == out.shape == (batch.tokens, heads, cache.head_dim)
-    need = paged_attention_workspace_size(cache, batch, q.dtype, heads)
+    stream = _raw_stream(cache.k, batch.first, q, out, workspace, err_flag)
+    assert q.dtype is out.dtype and q.shape == out.shape == (batch.tokens, heads, cache.head_dim) and out.is_contiguous()
+    assert err_flag is None or err_flag.dtype is torch.int32
+    handle, dtype = lib(), storage_of(q)
+    need = handle.rmlk_hip_paged_attention_workspace_size(dtype, cache.struct, batch.struct, heads)
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    check(lib().rmlk_hip_paged_attention(_stream(), storage_of(q), cache.struct, batch.struct, heads, q.data_ptr(),
-                                         _rows(q, heads * cache.head_dim), int(scale_is_mul), float(scale),
-                                         _ptr(workspace), ws_bytes, _ptr(out), _ptr(err_flag)),
-          "rmlk_hip_paged_attention")
+    ws_bytes = 0
+    if workspace is not None:
+        assert workspace.is_contiguous()
+        ws_bytes = workspace.numel() * workspace.element_size()
+    status = handle.rmlk_hip_paged_attention(stream, dtype, cache.struct, batch.struct, heads, q.data_ptr(),
+                                             _pitch(q, heads * cache.head_dim), int(scale_is_mul), scale,
+                                             _address(workspace), ws_bytes, out.data_ptr(), _address(err_flag))
+    if status:
+        check(status, "rmlk_hip_paged_attention")
 
 
 def memcpy_dtod_many(dsts, srcs) -> None:
