@@ -14,8 +14,10 @@ pub mod fused;
 pub mod gather;
 pub mod gemm;
 pub mod greater;
+pub mod int8;
 pub mod mul;
 pub mod neg;
+pub mod paged;
 pub mod pow;
 pub mod reduce_mean;
 pub mod scatter_nd;
