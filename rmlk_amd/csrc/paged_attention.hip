@@ -296,21 +296,35 @@ __device__ __forceinline__ void store_four(T *to, const f32x4 &o) {
     }
 }
 
-// Four neighbouring outputs of a row: the result, or (more than one split) a part of it with its statistics.
+// Where a row's outputs go: the result, or (more than one split) a part of it with its statistics.
 template <typename T, int D>
-__device__ __forceinline__ void put_output(const AttendArgs<T> &g, const Sequence &s, int kv, int r, int split, int d,
-                                           const f32x4 &o, float ref, float total) {
-    const int token = r / g.rep;
-    const int64_t at = (s.row + token) * static_cast<int64_t>(g.heads) + kv * g.rep + r % g.rep;
-    if (s.length - s.fresh + token + 1 <= g.chunk) {     // (all it sees lies in the first split)
-        if (split == 0) store_four(g.out + at * D + d, o);
-    } else {
+struct Output {
+    T *out;           // null: a part
+    float *part;
+    float2 *stats;
+    bool nothing;     // another split's
+
+    __device__ __forceinline__ Output(const AttendArgs<T> &g, const Sequence &s, int kv, int r, int split) {
+        const int token = r / g.rep;
+        const int64_t at = (s.row + token) * static_cast<int64_t>(g.heads) + kv * g.rep + r % g.rep;
+        const bool whole = s.length - s.fresh + token + 1 <= g.chunk;     // (all it sees lies in the first split)
         const int64_t all_rows = g.c.rows * g.heads;
-        *reinterpret_cast<f32x4 *>(g.part + (split * all_rows + at) * D + d) = o;
-        if (d == 0)
-            reinterpret_cast<float2 *>(g.part + g.splits * all_rows * D)[split * all_rows + at] = float2{ref, total};
+        nothing = whole && split > 0;
+        out = whole ? g.out + at * D : nullptr;
+        part = g.part + (split * all_rows + at) * D;
+        stats = reinterpret_cast<float2 *>(g.part + g.splits * all_rows * D) + split * all_rows + at;
     }
-}
+    // four neighbouring outputs
+    __device__ __forceinline__ void put(int d, const f32x4 &o, float ref, float total) const {
+        if (nothing) return;
+        if (out) {
+            store_four(out + d, o);
+        } else {
+            *reinterpret_cast<f32x4 *>(part + d) = o;
+            if (d == 0) *stats = float2{ref, total};
+        }
+    }
+};
 
 // The place of a block in the work: KV head, sequence, first row, split. False: nothing to do.
 struct Place {
@@ -481,7 +495,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
             o += *reinterpret_cast<const f32x4 *>(lds + (w * R + row) * kPad + d) * weight;
         }
         o *= total == 0.f ? 0.f : 1.f / total;
-        put_output<T, D>(g, p.s, p.kv, p.r0 + row, p.split, d, o, top, total);
+        Output<T, D>(g, p.s, p.kv, p.r0 + row, p.split).put(d, o, top, total);
     }
 }
 
@@ -506,7 +520,6 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     soft.clear();
     const int past = p.s.length - p.s.fresh;
     const int my_least = past + my_r0 / g.rep + 1;
-    const int my_end = my_r0 < p.rows ? min(p.end, past + min(my_r0 + 16 * NT - 1, p.rows - 1) / g.rep + 1) : 0;
 
     const int last_page = (p.s.length > 0 ? p.s.length - 1 : 0) >> g.c.page_shift;
     const int size = 1 << g.c.page_shift;
@@ -583,17 +596,17 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
                 fetch(raw, t1, a, b);
             }
             __syncthreads();      // this tile is in LDS, and the other buffer has been read by everyone
-            if (t0 < my_end) {
-                if (ready.step_exp > my_exp) {
-                    soft.rescale(ldexpf(1.f, my_exp - ready.step_exp));
-                    my_exp = ready.step_exp;
-                }
-                const u32x4 *from = frags + buf * kFrags * kWave + lane;
-                soft.tile(
-                    rows, [&](int j, int q) { return __builtin_bit_cast(h8, from[(j * KH + q) * kWave]); },
-                    [&](int d, int hh) { return __builtin_bit_cast(h8, from[(4 * KH + d * 2 + hh) * kWave]); }, ready.kc,
-                    t0, t1 > my_least || __any(ready.bad), ready.bad);
+            // (a wavefront whose rows see nothing of the tile goes along: the branch around it cost more, in copies
+            // of the accumulators where its two sides meet)
+            if (ready.step_exp > my_exp) {
+                soft.rescale(ldexpf(1.f, my_exp - ready.step_exp));
+                my_exp = ready.step_exp;
             }
+            const u32x4 *from = frags + buf * kFrags * kWave + lane;
+            soft.tile(
+                rows, [&](int j, int q) { return __builtin_bit_cast(h8, from[(j * KH + q) * kWave]); },
+                [&](int d, int hh) { return __builtin_bit_cast(h8, from[(4 * KH + d * 2 + hh) * kWave]); }, ready.kc, t0,
+                t1 > my_least || __any(ready.bad), ready.bad);
             buf ^= 1;
             if (more) ready = widen_tile(raw, buf);
         }
@@ -604,12 +617,13 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
         const float inv = total == 0.f ? 0.f : 1.f / total;
         const int r = my_r0 + n * 16 + col;
         if (r >= p.rows) continue;
+        const Output<T, D> out(g, p.s, p.kv, r, p.split);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             f32x4 o = soft.acc[d][n] * inv;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], my_exp);
-            put_output<T, D>(g, p.s, p.kv, r, p.split, d * 16 + grp * 4, o, soft.ref[n], total);
+            out.put(d * 16 + grp * 4, o, soft.ref[n], total);
         }
     }
 }
