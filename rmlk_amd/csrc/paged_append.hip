@@ -90,6 +90,32 @@ __device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
     for (size_t u = 0; u < sizeof(T) / 2; ++u) reinterpret_cast<u32x4 *>(to)[u] = reinterpret_cast<const u32x4 *>(v)[u];
 }
 
+// The same for a 16-bit result, in float: the rounding error of one product is carried along, so that nothing is
+// lost where the two cancel, and the result is off by 2^-23 of itself before it is rounded.
+__device__ __forceinline__ float two_products(float x, float c, float y, float s) {
+    const float p = y * s, rest = fmaf(y, s, -p);
+    return fmaf(x, c, p) + (fabsf(p) < INFINITY ? rest : 0.f);
+}
+template <typename T>
+__device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[8], const float (&b)[8], const Turn &t,
+                                              bool turn) {
+    if constexpr (sizeof(T) == 4) {
+        double lo[8], hi[8];
+        rotate_eight(a, b, t, turn, lo, hi);
+        store_eight(to, lo);
+        store_eight(to + half, hi);
+    } else {
+        T lo[8], hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lo[i] = static_cast<T>(turn ? two_products(a[i], t.c0[i], -b[i], t.s0[i]) : a[i]);
+            hi[i] = static_cast<T>(turn ? two_products(b[i], t.c1[i], a[i], t.s1[i]) : b[i]);
+        }
+        *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<const u32x4 *>(lo);
+        *reinterpret_cast<u32x4 *>(to + half) = *reinterpret_cast<const u32x4 *>(hi);
+    }
+}
+
 // Blocks 0 .. pieces * kv_heads - 1: a block takes one page of one sequence and KV head, K and V. Its threads
 // load all new values of it at once (PK units of 8 + 8 rotating dims of K, 2 PK units of 8 dims of V each),
 // agree on the two largest magnitudes and write: one trip over the values. V is turned in LDS when more
@@ -130,12 +156,7 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
             if (g.cos) load_turn<D>(turn, g.cos, g.sin, pos, d);
 #pragma unroll
             for (int i = 0; i < kHeads; ++i)
-                if (h0 + i < g.heads) {
-                    double lo[8], hi[8];
-                    rotate_eight(x[i][0], x[i][1], turn, g.cos != nullptr, lo, hi);
-                    store_eight(to + (h0 + i) * D, lo);
-                    store_eight(to + (h0 + i) * D + D / 2, hi);
-                }
+                if (h0 + i < g.heads) store_rotated(to + (h0 + i) * D, D / 2, x[i][0], x[i][1], turn, g.cos != nullptr);
         }
         return;
     }
