@@ -152,6 +152,34 @@ struct Rows {
     }
 };
 
+// The cache as one KV head of one sequence sees it. Addresses are a 32-bit page times a 32-bit pitch (at most
+// 65535 heads of 16 KB) behind a base that is the same in all lanes: one wide multiply each.
+template <int D>
+struct View {
+    const int8_t *k, *v;
+    const float *k_scale, *v_scale;
+    const int32_t *table;
+    uint32_t pages, pitch, heads;
+    int shift, size, last_page;
+    template <typename T>
+    __device__ __forceinline__ View(const AttendArgs<T> &g, const Sequence &s, int seq, int kv)
+        : k(g.c.k), v(g.c.v), k_scale(g.c.k_scale + kv), v_scale(g.c.v_scale + kv),
+          table(g.c.table + seq * g.c.table_stride), pages(static_cast<uint32_t>(g.c.pages)), heads(g.c.kv_heads),
+          shift(g.c.page_shift), size(1 << g.c.page_shift), last_page((s.length > 0 ? s.length - 1 : 0) >> shift) {
+        k += kv * size * D;
+        v += kv * size * D;
+        pitch = heads * static_cast<uint32_t>(size * D);
+    }
+    __device__ __forceinline__ uint32_t page_of(int token) const {
+        return static_cast<uint32_t>(table[static_cast<uint32_t>(min(token >> shift, last_page))]);
+    }
+    __device__ __forceinline__ bool has(uint32_t page) const { return page < pages; }
+    __device__ __forceinline__ const int8_t *at(const int8_t *base, uint32_t page, uint32_t offset) const {
+        return base + static_cast<uint64_t>(page) * pitch + offset;
+    }
+    __device__ __forceinline__ uint64_t scale_at(uint32_t page) const { return static_cast<uint64_t>(page) * heads; }
+};
+
 // What a wavefront has of its rows' softmax: outputs (times 2^-E), sums, reference points.
 template <typename T, int D, int NT>
 struct Softmax {
@@ -174,26 +202,10 @@ struct Softmax {
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[d][n] *= f;
     }
-    // One tile: k_frag(jj, h) and v_frag(d, hh) give the operands, kc K's step of the lane group's tokens;
-    // t0 the tile's first token, masked whether any row of the wavefront does not see all of it, bad whether the
-    // lane group's tokens are hidden from everyone. A hidden score becomes -inf before it is scaled: factors
-    // are kept positive, and where a row sees none of the lane group's tokens its factor is replaced, so that
-    // a step that is no number reaches only the rows that see the block.
-    template <typename KF, typename VF>
-    __device__ __forceinline__ void tile(const Rows<T, D, NT> &rows, KF &&k_frag, VF &&v_frag, float kc, int t0,
-                                         bool masked, bool bad) {
-        const int grp = threadIdx.x % kWave / 16;
-        float c[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            c[n] = rows.factor[n] * kc;
-            c[n] = c[n] < kLeastFactor ? kLeastFactor : c[n];
-        }
-        if (masked) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) c[n] = rows.limit[n] <= t0 + grp * 16 || bad ? kLeastFactor : c[n];
-        }
-        f32x4 sc[4][NT];
+    // S^T of a tile: k_frag(jj, h) gives K's operands.
+    typedef f32x4 Scores[4][NT];
+    template <typename KF>
+    __device__ __forceinline__ void scores(const Rows<T, D, NT> &rows, KF &&k_frag, Scores &sc) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -208,31 +220,45 @@ struct Softmax {
                         sc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, rows.q[p][n][q], sc[j][n], 0, 0, 0);
             }
         }
-        if (masked) {
-            const int key = t0 + grp * 16;
+    }
+    // Hides what a row does not see and moves the reference point where a score lies too far above it; c: the factors
+    // of the scores. kc is K's step of the lane group's tokens, t0 the tile's first token, masked whether any row of
+    // the wavefront does not see all of it, bad whether the lane group's tokens are hidden from everyone. A hidden
+    // score becomes -inf before it is scaled: factors are kept positive, and where a row sees none of the lane
+    // group's tokens its factor is replaced, so that a step that is no number reaches only the rows that see the
+    // block.
+    __device__ __forceinline__ void refer(const Rows<T, D, NT> &rows, Scores &sc, float (&c)[NT], float kc, int t0,
+                                          bool masked, bool bad) {
+        const int key = t0 + threadIdx.x % kWave / 16 * 16;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+            c[n] = rows.factor[n] * kc;
+            c[n] = c[n] < kLeastFactor ? kLeastFactor : c[n];
+        }
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                c[n] = rows.limit[n] <= key || bad ? kLeastFactor : c[n];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     sc[i / 4][n][i % 4] = key + i < rows.limit[n] && !bad ? sc[i / 4][n][i % 4] : -INFINITY;
+            }
         }
-        // exponents relative to the reference point (which is finite: a hidden score stays -inf)
-        auto exponent = [&](int n, int i) { return fmaf(sc[i / 4][n][i % 4], c[n], -ref[n]); };
+        // (factors are positive: the largest score has the largest exponent; the reference point is finite, so that
+        // the exponent of a hidden score stays -inf)
+        float top[NT];
         bool beyond = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float top = -INFINITY;
+            top[n] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, exponent(n, i));
-            beyond = top > kMostWeight || beyond;
+            for (int i = 0; i < 16; ++i) top[n] = fmaxf(top[n], sc[i / 4][n][i % 4]);
+            beyond = fmaf(top[n], c[n], -ref[n]) > kMostWeight || beyond;
         }
         if (__any(beyond)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i / 4][n][i % 4] * c[n]);
-                const float now = fmaxf(ref[n], across_groups_max(top) - kBase);
+                const float now = fmaxf(ref[n], across_groups_max(top[n] * c[n]) - kBase);
                 const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
                 ref[n] = now;
                 sum[n] *= alpha;
@@ -240,39 +266,59 @@ struct Softmax {
                 for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
             }
         }
+    }
+    // The weights of half hh of a tile, as P^T operands.
+    typedef h8 Weights[P][NT];
+    __device__ __forceinline__ void weights(const Scores &sc, const float (&c)[NT], int hh, Weights &pf) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const f32x4 &four = sc[hh * 2 + i / 4][n];
+                const f32x2 w = {__builtin_amdgcn_exp2f(fmaf(four[i % 4], c[n], -ref[n])),
+                                 __builtin_amdgcn_exp2f(fmaf(four[i % 4 + 1], c[n], -ref[n]))};
+                const h2 hi = __builtin_convertvector(w, h2);
+                pf[0][n][i] = hi[0];
+                pf[0][n][i + 1] = hi[1];
+                if constexpr (P == 2) {
+                    sum[n] += w[0];
+                    sum[n] += w[1];
+                    const f32x2 rest = {w[0] - static_cast<float>(hi[0]), w[1] - static_cast<float>(hi[1])};
+                    const h2 lo = __builtin_convertvector(rest, h2);
+                    pf[1][n][i] = lo[0];
+                    pf[1][n][i + 1] = lo[1];
+                } else {
+                    // (the sum of the weights as they are multiplied: their rounding cancels in part)
+                    sum[n] = __builtin_amdgcn_fdot2(hi, h2{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, sum[n], false);
+                }
+            }
+    }
+    // O^T of half hh of a tile: v_frag(d, hh) gives V's operands.
+    template <typename VF>
+    __device__ __forceinline__ void outputs(VF &&v_frag, int hh, const Weights &pf) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const h8 va = v_frag(d, hh);
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
+        }
+    }
+    // One tile from beginning to end.
+    template <typename KF, typename VF>
+    __device__ __forceinline__ void tile(const Rows<T, D, NT> &rows, KF &&k_frag, VF &&v_frag, float kc, int t0,
+                                         bool masked, bool bad) {
+        Scores sc;
+        float c[NT];
+        scores(rows, k_frag, sc);
+        refer(rows, sc, c, kc, t0, masked, bad);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-            h8 pf[P][NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const f32x2 w = {__builtin_amdgcn_exp2f(exponent(n, hh * 8 + i)),
-                                     __builtin_amdgcn_exp2f(exponent(n, hh * 8 + i + 1))};
-                    const h2 hi = __builtin_convertvector(w, h2);
-                    pf[0][n][i] = hi[0];
-                    pf[0][n][i + 1] = hi[1];
-                    if constexpr (P == 2) {
-                        sum[n] += w[0];
-                        sum[n] += w[1];
-                        const f32x2 rest = {w[0] - static_cast<float>(hi[0]), w[1] - static_cast<float>(hi[1])};
-                        const h2 lo = __builtin_convertvector(rest, h2);
-                        pf[1][n][i] = lo[0];
-                        pf[1][n][i + 1] = lo[1];
-                    } else {
-                        // (the sum of the weights as they are multiplied: their rounding cancels in part)
-                        sum[n] = __builtin_amdgcn_fdot2(hi, h2{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, sum[n], false);
-                    }
-                }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const h8 va = v_frag(d, hh);
-#pragma unroll
-                for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
-            }
+            Weights pf;
+            weights(sc, c, hh, pf);
+            outputs(v_frag, hh, pf);
         }
     }
 };
@@ -387,30 +433,28 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     soft.clear();
     int step_exp = -200;       // E: log2 of the largest step of V met so far
 
-    const int last_page = (p.s.length > 0 ? p.s.length - 1 : 0) >> g.c.page_shift;
-    const int size = 1 << g.c.page_shift;
-    const int32_t *table = g.c.table + p.seq * g.c.table_stride;
+    const View<D> view(g, p.s, p.seq, p.kv);
     // pages of the tokens whose K rows (by lane column) and whose V columns (by lane group) a lane loads
-    auto pages_of = [&](int t0, int32_t &pk, int32_t &pv) {
-        pk = table[min((t0 + (col / 4) * 16) >> g.c.page_shift, last_page)];
-        pv = table[min((t0 + grp * 16) >> g.c.page_shift, last_page)];
+    auto pages_of = [&](int t0, uint32_t &pk, uint32_t &pv) {
+        pk = view.page_of(t0 + (col / 4) * 16);
+        pv = view.page_of(t0 + grp * 16);
     };
-    auto fetch = [&](Tile<D> &t, int t0, int32_t pk, int32_t pv) {
-        t.bad = pv < 0 || pv >= g.c.pages;
+    auto fetch = [&](Tile<D> &t, int t0, uint32_t pk, uint32_t pv) {
+        t.bad = !view.has(pv);
         if (t.bad) raise_error(g.c);
-        pk = pk < 0 || pk >= g.c.pages ? 0 : pk;
+        pk = view.has(pk) ? pk : 0;
         pv = t.bad ? 0 : pv;
-        const int64_t bk = static_cast<int64_t>(pk) * g.c.kv_heads + p.kv, bv = static_cast<int64_t>(pv) * g.c.kv_heads + p.kv;
-        const int8_t *k = g.c.k + (bk * size + ((t0 + (col / 4) * 16 + col % 4) & (size - 1))) * D + grp * 16;
-        const int8_t *v = g.c.v + bv * size * D + ((t0 + grp * 16) & (size - 1)) + static_cast<int64_t>(col) * size;
-        t.k_scale = g.c.k_scale[bv];
-        t.v_scale = g.c.v_scale[bv];
+        const int mask = view.size - 1;
+        const int8_t *k = view.at(view.k, pk, ((t0 + (col / 4) * 16 + col % 4) & mask) * D + grp * 16);
+        const int8_t *v = view.at(view.v, pv, ((t0 + grp * 16) & mask) + col * view.size);
+        t.k_scale = view.k_scale[view.scale_at(pv)];
+        t.v_scale = view.v_scale[view.scale_at(pv)];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int c = 0; c < KC; ++c) t.k[j][c] = *reinterpret_cast<const u32x4 *>(k + j * 4 * D + c * 64);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + static_cast<int64_t>(d) * 16 * size);
+        for (int d = 0; d < DT; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + d * 16 * view.size);
     };
     auto compute = [&](const Tile<D> &t, int t0) {
         // V's steps relative to the largest; a step that is no number marks the scores instead
@@ -440,9 +484,9 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     int t0 = p.begin + wave * kTileKeys;
     if (t0 < p.end) {
         Tile<D> one, two;
-        int32_t pk, pv;
+        uint32_t pk, pv;
         pages_of(t0, pk, pv);
-        int32_t next_pk = 0, next_pv = 0;
+        uint32_t next_pk = 0, next_pv = 0;
         if (t0 + kStride < p.end) pages_of(t0 + kStride, next_pk, next_pv);
         fetch(one, t0, pk, pv);
         while (true) {
@@ -450,7 +494,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
                 const int t1 = t0 + kStride, t2 = t1 + kStride;
                 const bool more = t1 < p.end;
                 if (more) {
-                    const int32_t a = next_pk, b = next_pv;
+                    const uint32_t a = next_pk, b = next_pv;
                     if (t2 < p.end) pages_of(t2, next_pk, next_pv);
                     fetch(next, t1, a, b);
                 }
@@ -507,8 +551,7 @@ constexpr int kManyWaves = 4;
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(AttendArgs<T> g) {
     constexpr int DT = D / 16, KC = D / 64, KH = D / 32, R = 16 * NT * kManyWaves, DW = DT / kManyWaves;
-    constexpr int kFrags = 4 * KH + 2 * DT;        // of a tile: K's [4][KH], then V's [DT][2]
-    extern __shared__ __align__(16) u32x4 frags[];   // [2][kFrags][64 lanes]
+    extern __shared__ __align__(16) u32x4 frags[];   // K [2][4][KH][64 lanes], V [2][DT][2][64 lanes]
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int col = lane % 16, grp = lane / 16;
     Place p;
@@ -521,94 +564,119 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     const int past = p.s.length - p.s.fresh;
     const int my_least = past + my_r0 / g.rep + 1;
 
-    const int last_page = (p.s.length > 0 ? p.s.length - 1 : 0) >> g.c.page_shift;
-    const int size = 1 << g.c.page_shift;
-    const int32_t *table = g.c.table + p.seq * g.c.table_stride;
+    const View<D> view(g, p.s, p.seq, p.kv);
     // a quarter of a tile: the K rows of one S^T block, DW row blocks of V
     struct Raw {
         u32x4 k[KC], v[DW];
-        float k_scale, v_scale;
+        float k_scale, v_scale;       // of V's tile
         bool bad;
     };
-    auto pages_of = [&](int t0, int32_t &pk, int32_t &pv) {
-        pk = table[min((t0 + (col / 4) * 16) >> g.c.page_shift, last_page)];
-        pv = table[min((t0 + grp * 16) >> g.c.page_shift, last_page)];
-    };
-    auto fetch = [&](Raw &t, int t0, int32_t pk, int32_t pv) {
-        t.bad = pv < 0 || pv >= g.c.pages;
-        if (t.bad) raise_error(g.c);
-        pk = pk < 0 || pk >= g.c.pages ? 0 : pk;
-        pv = t.bad ? 0 : pv;
-        const int64_t bk = static_cast<int64_t>(pk) * g.c.kv_heads + p.kv, bv = static_cast<int64_t>(pv) * g.c.kv_heads + p.kv;
-        const int8_t *k = g.c.k + (bk * size + ((t0 + (col / 4) * 16 + wave * 4 + col % 4) & (size - 1))) * D + grp * 16;
-        const int8_t *v = g.c.v + bv * size * D + ((t0 + grp * 16) & (size - 1)) +
-                          static_cast<int64_t>(wave * DW * 16 + col) * size;
-        t.k_scale = g.c.k_scale[bv];
-        t.v_scale = g.c.v_scale[bv];
+    auto k_page = [&](int t0) { return view.page_of(t0 + (col / 4) * 16); };
+    auto v_page = [&](int t0) { return view.page_of(t0 + grp * 16); };
+    auto fetch_k = [&](Raw &t, int t0, uint32_t page) {
+        const int8_t *k = view.at(view.k, view.has(page) ? page : 0,
+                                  ((t0 + (col / 4) * 16 + wave * 4 + col % 4) & (view.size - 1)) * D + grp * 16);
 #pragma unroll
         for (int c = 0; c < KC; ++c) t.k[c] = *reinterpret_cast<const u32x4 *>(k + c * 64);
-#pragma unroll
-        for (int d = 0; d < DW; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + static_cast<int64_t>(d) * 16 * size);
     };
-    // the tile in LDS and what every wavefront knows of it
+    auto fetch_v = [&](Raw &t, int t0, uint32_t page) {
+        t.bad = !view.has(page);
+        if (t.bad) raise_error(g.c);
+        page = t.bad ? 0 : page;
+        const int8_t *v = view.at(view.v, page, ((t0 + grp * 16) & (view.size - 1)) + (wave * DW * 16 + col) * view.size);
+        t.k_scale = view.k_scale[view.scale_at(page)];
+        t.v_scale = view.v_scale[view.scale_at(page)];
+#pragma unroll
+        for (int d = 0; d < DW; ++d) t.v[d] = *reinterpret_cast<const u32x4 *>(v + d * 16 * view.size);
+    };
+    // what every wavefront knows of a tile whose V is in LDS
     struct Ready {
         float kc;
         int step_exp;
         bool bad;
     };
     int step_exp = -200;       // E: log2 of the largest step of V met so far, the same in all wavefronts
-    auto widen_tile = [&](const Raw &t, int buf) {
-        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
-        step_exp = max(step_exp, largest_step(t.v_scale, odd));
-        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
-        const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
-        const h2 vf = {f1, f1}, vbias = {b1, b1};
-        u32x4 *to = frags + buf * kFrags * kWave + lane;
+    constexpr int kKFrags = 4 * KH, kVFrags = 2 * DT;
+    u32x4 *const k_lds = frags + lane, *const v_lds = frags + 2 * kKFrags * kWave + lane;
+    auto widen_k = [&](const Raw &t, int buf) {
+        u32x4 *to = k_lds + buf * kKFrags * kWave;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             to[(wave * KH + 2 * c) * kWave] = __builtin_bit_cast(u32x4, widen(t.k[c][0], t.k[c][1]));
             to[(wave * KH + 2 * c + 1) * kWave] = __builtin_bit_cast(u32x4, widen(t.k[c][2], t.k[c][3]));
         }
+    };
+    auto widen_v = [&](const Raw &t, int buf) {
+        const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
+        step_exp = max(step_exp, largest_step(t.v_scale, odd));
+        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
+        const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
+        const h2 vf = {f1, f1}, vbias = {b1, b1};
+        u32x4 *to = v_lds + buf * kVFrags * kWave;
 #pragma unroll
         for (int d = 0; d < DW; ++d)
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh)
-                to[(4 * KH + (wave * DW + d) * 2 + hh) * kWave] =
+                to[((wave * DW + d) * 2 + hh) * kWave] =
                     __builtin_bit_cast(u32x4, widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias));
         return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, step_exp, t.bad};
     };
 
     int my_exp = -200;
     if (p.begin < p.end) {
+        // K is one tile ahead of V: a tile's scores are computed beside the weights of the tile before it, so that
+        // the matrix cores and the other units have work at the same time. (Past the last tile the scores are of
+        // what the buffer happens to hold, and are not used.)
         Raw raw;
-        int32_t pk, pv;
-        pages_of(p.begin, pk, pv);
-        fetch(raw, p.begin, pk, pv);
-        if (p.begin + kTileKeys < p.end) pages_of(p.begin + kTileKeys, pk, pv);
-        Ready ready = widen_tile(raw, 0);
-        int buf = 0;
+        fetch_k(raw, p.begin, k_page(p.begin));
+        fetch_v(raw, p.begin, v_page(p.begin));
+        Ready ready = widen_v(raw, 0);
+        widen_k(raw, 0);
+        if (p.begin + kTileKeys < p.end) {
+            fetch_k(raw, p.begin + kTileKeys, k_page(p.begin + kTileKeys));
+            widen_k(raw, 1);
+        }
+        uint32_t pk = k_page(p.begin + 2 * kTileKeys), pv = v_page(p.begin + kTileKeys);
+        int buf = 0;        // of this tile
+        typename Softmax<T, D, NT>::Scores sc;
+        auto score = [&](int from, typename Softmax<T, D, NT>::Scores &to) {
+            const u32x4 *k = k_lds + from * kKFrags * kWave;
+            soft.scores(rows, [&](int j, int q) { return __builtin_bit_cast(h8, k[(j * KH + q) * kWave]); }, to);
+        };
+        __syncthreads();
+        score(0, sc);
         for (int t0 = p.begin; t0 < p.end; t0 += kTileKeys) {
-            const int t1 = t0 + kTileKeys;
-            const bool more = t1 < p.end;
-            if (more) {
-                const int32_t a = pk, b = pv;
-                if (t1 + kTileKeys < p.end) pages_of(t1 + kTileKeys, pk, pv);
-                fetch(raw, t1, a, b);
-            }
-            __syncthreads();      // this tile is in LDS, and the other buffer has been read by everyone
+            const int t1 = t0 + kTileKeys, t2 = t1 + kTileKeys;
+            fetch_v(raw, t1, pv);
+            fetch_k(raw, t2, pk);
+            pk = k_page(t2 + kTileKeys);
+            pv = v_page(t2);
+            __syncthreads();      // V of this tile and K of the next are in LDS, the other buffers have been read by everyone
             // (a wavefront whose rows see nothing of the tile goes along: the branch around it cost more, in copies
             // of the accumulators where its two sides meet)
             if (ready.step_exp > my_exp) {
                 soft.rescale(ldexpf(1.f, my_exp - ready.step_exp));
                 my_exp = ready.step_exp;
             }
-            const u32x4 *from = frags + buf * kFrags * kWave + lane;
-            soft.tile(
-                rows, [&](int j, int q) { return __builtin_bit_cast(h8, from[(j * KH + q) * kWave]); },
-                [&](int d, int hh) { return __builtin_bit_cast(h8, from[(4 * KH + d * 2 + hh) * kWave]); }, ready.kc, t0,
-                t1 > my_least || __any(ready.bad), ready.bad);
+            float c[NT];
+            soft.refer(rows, sc, c, ready.kc, t0, t1 > my_least || __any(ready.bad), ready.bad);
+            const u32x4 *v = v_lds + buf * kVFrags * kWave;
+            auto v_frag = [&](int d, int hh) { return __builtin_bit_cast(h8, v[(d * 2 + hh) * kWave]); };
+            typename Softmax<T, D, NT>::Weights pf[2];
+            typename Softmax<T, D, NT>::Scores next;
+            score(buf ^ 1, next);
+            soft.weights(sc, c, 0, pf[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            soft.weights(sc, c, 1, pf[1]);
+            soft.outputs(v_frag, 0, pf[0]);
+            soft.outputs(v_frag, 1, pf[1]);
+            ready = widen_v(raw, buf ^ 1);
+            widen_k(raw, buf);
             buf ^= 1;
-            if (more) ready = widen_tile(raw, buf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[j][n] = next[j][n];
         }
     }
 #pragma unroll
