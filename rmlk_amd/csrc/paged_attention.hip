@@ -664,12 +664,19 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
             auto v_frag = [&](int d, int hh) { return __builtin_bit_cast(h8, v[(d * 2 + hh) * kWave]); };
             typename Softmax<T, D, NT>::Weights pf[2];
             typename Softmax<T, D, NT>::Scores next;
-            score(buf ^ 1, next);
-            soft.weights(sc, c, 0, pf[0]);
-            __builtin_amdgcn_sched_barrier(0);
-            soft.weights(sc, c, 1, pf[1]);
-            soft.outputs(v_frag, 0, pf[0]);
-            soft.outputs(v_frag, 1, pf[1]);
+            if constexpr (Softmax<T, D, NT>::P * D < 256) {
+                score(buf ^ 1, next);
+                soft.weights(sc, c, 0, pf[0]);
+                soft.weights(sc, c, 1, pf[1]);
+                soft.outputs(v_frag, 0, pf[0]);
+                soft.outputs(v_frag, 1, pf[1]);
+            } else {
+                soft.weights(sc, c, 0, pf[0]);
+                soft.outputs(v_frag, 0, pf[0]);
+                soft.weights(sc, c, 1, pf[1]);
+                soft.outputs(v_frag, 1, pf[1]);
+                score(buf ^ 1, next);
+            }
             ready = widen_v(raw, buf ^ 1);
             widen_k(raw, buf);
             buf ^= 1;
