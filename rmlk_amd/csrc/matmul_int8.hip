@@ -466,7 +466,9 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args<T> g, int32_t s
 
 template <typename T, int MT, int WAVES>
 int32_t launch_few_rows(hipStream_t st, const Int8Args<T> &g) {
-    int8_few_rows_kernel<T, MT, WAVES><<<static_cast<uint32_t>((g.n + 15) / 16), WAVES * kWave, 0, st>>>(g);
+    const int64_t blocks = (static_cast<int64_t>(g.n) + 15) / 16;
+    if (blocks * (WAVES * kWave) >= (static_cast<int64_t>(1) << 32)) return RMLK_ERR_TOO_LARGE;    // work items of a launch
+    int8_few_rows_kernel<T, MT, WAVES><<<static_cast<uint32_t>(blocks), WAVES * kWave, 0, st>>>(g);
     return launch_status();
 }
 
@@ -503,7 +505,7 @@ struct Plan {
 Plan plan_for(int64_t m, int64_t n, int64_t k) {
     auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
     Plan p{kTile64, 1, static_cast<int32_t>(k)};
-    if (m > 4 && m <= 32 && n >= 64 * kNumCU && k <= 4096) {
+    if (m > 4 && m <= 32 && n >= 64 * kNumCU && k > 0 && k <= 4096) {
         p.route = kWide;
     } else if (m <= 16 || (m <= 32 && n * k <= (1 << 23))) {
         p.route = kFewRows;

@@ -385,6 +385,7 @@ int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_pa
     if (k_stride % unit || v_stride % unit || (q && q_stride % unit) || !aligned16(k) || !aligned16(v) ||
         !aligned16(q) || !aligned16(q_out) || !aligned16(cos) || !aligned16(sin))
         return RMLK_ERR_UNSUPPORTED;
+    if (q && q == q_out && q_stride != heads * d) return RMLK_ERR_INVALID_ARGUMENT;   // (rows would move under their readers)
     const int64_t pieces = (c.rows >> c.page_shift) + 2 * c.seqs;
     if (pieces * c.kv_heads > (1 << 23)) return RMLK_ERR_TOO_LARGE;
     return with_activation(dtype, [&](auto tag) {

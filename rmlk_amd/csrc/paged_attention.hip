@@ -765,8 +765,9 @@ Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
     p.many = rows > 32;
     p.nt = p.many ? 2 : rows <= 16 || head_dim == 128 ? 1 : 2;
     const int64_t tile = 16 * p.nt * (p.many ? kManyWaves : 1);
-    // upper bound of the row tiles; exact where all sequences bring the same rows
-    const int64_t ragged = c.rows * rep / tile + c.seqs, even = c.seqs * ((rows + tile - 1) / tile);
+    // upper bound of the row tiles; exact where all sequences bring the same rows (a sequence that brings more than
+    // the call allows, be that none, is a tile that reports it)
+    const int64_t ragged = c.rows * rep / tile + c.seqs, even = c.seqs * (rows > 0 ? (rows + tile - 1) / tile : 1);
     p.pieces = ragged < even ? ragged : even;
     const int64_t step = kTileKeys * (p.many ? 1 : kFewWaves);
     const int64_t len = c.max_length > 0 ? c.max_length : 1;

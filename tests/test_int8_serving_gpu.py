@@ -212,6 +212,23 @@ def test_matmul_int8_largest_sums(device):
     assert np.array_equal(_f64(out), np.broadcast_to(want.astype(np.float32), (2, 20)))
 
 
+@pytest.mark.parametrize("m,n", [(1, 48), (8, 16400), (20, 17000), (40, 96), (300, 520)])
+def test_matmul_int8_without_columns(device, m, n):
+    """k = 0, on every route a size can take: the sums are empty, nothing is read of either operand."""
+    from rmlk_amd._lib import lib
+    one_m, one_n = torch.ones(m, device=device), torch.ones(n, device=device)
+    res = torch.randn(m, n, device=device)
+    a, w = (torch.full((r, 16), 99, dtype=torch.int8, device=device) for r in (m, n))
+    for residual, want in ((None, torch.zeros_like(res)), (res, res)):
+        out = torch.full_like(res, float("nan"))
+        _k().matmul_int8(a, one_m, w, one_n, out, k=0, residual=residual)
+        assert torch.equal(out, want)
+    out = torch.full_like(res, float("nan"))
+    status = lib().rmlk_hip_matmul_int8(torch.cuda.current_stream().cuda_stream, 1, m, n, 0, 0, 0, one_m.data_ptr(), 0, 0,
+                                        one_n.data_ptr(), res.data_ptr(), n, 0, 0, out.data_ptr(), n)
+    assert status == 0 and torch.equal(out, res)
+
+
 def test_matmul_int8_scale_that_is_not_a_number_stays_in_its_row(device):
     rng = np.random.default_rng(2)
     for m in (4, 70):
@@ -369,6 +386,33 @@ def test_paged_append_not_finite_values_mark_their_block(device):
     many = np.ones((20, 2, 64), np.float32)
     _append(p, "f32", [20], [20], values=(many, many), rotate=False, with_q=False)   # started anew
     assert not np.isnan(p.ref.k_scale).any()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_paged_append_rotates_queries_that_are_not_finite_or_large(device, kind):
+    """Infinities, NaN and the type's largest values go where the formula sends them, and only there."""
+    kk = _k()
+    p = Paged(device, 1, 16, 1, 64, 16, 12)
+    dt = TYPES[kind]
+    most = torch.finfo(dt).max
+    q = torch.ones(6, 2, 64, device=device, dtype=dt)
+    for i, value in enumerate((float("inf"), -float("inf"), float("nan"), most, -most)):
+        q[i, 0, 3] = value          # the first half of the row
+        q[i, 1, 35] = value         # the second
+    kv = torch.ones(6, 1, 64, device=device, dtype=dt)
+    cos, sin = (_dev(t, device) for t in _tables(np.random.default_rng(1), 6, 64))
+    out = torch.zeros_like(q)
+    kk.paged_append(p.dev, p.batch([0, 6], [6], 6, 6, 6), kv, kv, cos=cos, sin=sin, q=q, q_out=out)
+    x, c, s = _f64(q), _f64(cos)[:, None], _f64(sin)[:, None]
+    turned = np.concatenate([-x[..., 32:], x[..., :32]], axis=-1)
+    with np.errstate(all="ignore"):
+        want = x * c + turned * s
+    got, bound = _f64(out), float(most)
+    nan, inside = np.isnan(want), np.abs(want) < bound
+    assert np.array_equal(np.isnan(got), nan)
+    beyond = ~nan & ~inside          # (the largest value or an infinity: one rounding apart)
+    assert np.all(np.sign(got[beyond]) == np.sign(want[beyond])) and np.all(np.abs(got[beyond]) >= bound)
+    assert np.all(np.abs(got[inside] - want[inside]) <= 1.01 * U_OUT[kind] * np.abs(want[inside]) + TINY[kind])
 
 
 def test_paged_append_bad_numbers_are_reported_and_skipped(device):
@@ -636,6 +680,23 @@ def test_paged_attention_bad_numbers_are_reported_and_skipped(device):
             want, bound = ref.attend(q64[3 + i:4 + i, h], k[see], v[see], len(see), 0.125)
             tol = (4 * (2.0 ** -22 + 68 * U) * bound[0] + 64 * U) * np.abs(v).max() + U * np.abs(want)
             assert np.all(np.abs(_f64(out[3 + i, h]) - want[0]) <= tol[0])
+
+
+def test_paged_calls_of_a_padded_batch_without_new_tokens(device):
+    """Rows, but none of them a sequence's (max_new 0): nothing is written; a sequence that has some is reported."""
+    kk = _k()
+    p = Paged(device, 3, 16, 2, 64, 64, 47)
+    x = torch.ones(9, 2, 64, device=device)
+    for max_len in (64, 1 << 20):
+        for first, bad in (([0, 0, 0, 0], 0), ([4, 4, 4, 4], 0), ([0, 0, 2, 2], 1)):
+            flag = torch.zeros(2, dtype=torch.int32, device=device)
+            out = torch.full((9, 4, 64), 7.0, device=device)
+            batch = kk.PagedBatch(_dev(np.asarray(first, np.int32), device), _dev(np.asarray([20, 20, 0], np.int32), device),
+                                  _dev(p.table, device), tokens=9, max_new=0, max_len=max_len)
+            kk.paged_append(p.dev, batch, x, x, err_flag=flag[:1])
+            kk.paged_attention(p.dev, batch, torch.ones_like(out), out, scale=0.125, err_flag=flag[1:])
+            assert flag.tolist() == [bad, bad] and bool((out == 7).all())
+            p.check_cache()
 
 
 def test_paged_attention_sequences_that_share_pages(device):

@@ -149,3 +149,26 @@ def test_paged_attention(L):
     assert size(DOUBLE, ctypes.byref(_cache()), ctypes.byref(_batch(**long)), 4) == 0
     assert size(FLOAT, ctypes.byref(_cache()), ctypes.byref(_batch(seqs=0, **long)), 4) == 0
     assert size(FLOAT, None, None, 4) == 0
+
+
+def test_sizes_beyond_a_launch(L):
+    """More channels than a launch has work items for."""
+    n = (1 << 27) + 16
+    assert L.rmlk_hip_matmul_int8(None, FLOAT, 1, n, 16, P, 16, P, P, 16, P, 0, 0, 0, 0, P, n) == TOO_LARGE
+
+
+def test_paged_append_rotation_in_place_needs_dense_rows(L):
+    """q_out is dense: over a q whose rows lie apart it would overwrite rows that are still to be read."""
+    def call(q_out, stride):
+        return L.rmlk_hip_paged_append(None, FLOAT, ctypes.byref(_cache()), ctypes.byref(_batch(rows=4)), P, 128, P, 128, 0, 0,
+                                       0, 4, P, stride, q_out, 0)
+    assert call(P, 512) == INVALID_ARGUMENT and call(P, 260) == INVALID_ARGUMENT
+
+
+def test_paged_attention_workspace_without_new_tokens(L):
+    """max_new 0 (a padded batch): an answer, whatever the lengths."""
+    size = L.rmlk_hip_paged_attention_workspace_size
+    for max_length in (0, 40, 5000, 100000):
+        for seqs in (1, 2, 70):
+            b = _batch(seqs=seqs, max_new=0, max_length=max_length, table_stride=7000)
+            assert size(FLOAT, ctypes.byref(_cache()), ctypes.byref(b), 4) >= 0
