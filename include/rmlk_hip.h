@@ -657,7 +657,8 @@ int32_t rmlk_hip_gemv_kmajor_head_rows(rmlk_stream_t stream, int32_t dtype, int6
  * decided as in exact arithmetic; |q| <= 127. A row whose largest magnitude lies below 2^-100 gets
  * scale 0 and q 0; a row that holds a NaN or an infinity gets scale NaN and q 0, so that what is
  * computed from it is NaN. x has rows of `cols` values ldx apart, q rows ldq bytes apart with ldq a
- * multiple of 16, ldq >= cols; bytes cols .. cols rounded up to 16 of a row are set to zero.
+ * multiple of 16, ldq >= cols; bytes cols .. cols rounded up to 16 of a row are set to zero. Rows of no
+ * columns: nothing is written.
  * rmlk_hip_rmsnorm_quantize_rows: the same of y = x / sqrt(mean(x^2) + eps) * gamma (evaluated in
  * double), with b given of x + b, which is rounded to `dtype`, stored to sum_out and normalised from
  * there. x, b, sum_out dense [rows, cols] (sum_out may be x or b), gamma float [cols]; b and sum_out
@@ -671,11 +672,13 @@ int32_t rmlk_hip_rmsnorm_quantize_rows(rmlk_stream_t stream, int32_t dtype, int6
 
 /* c[i, j] = (sum_k a[i, k] * wt[j, k]) * a_scale[i] * w_scale[j] (+ residual[i, j]), rounded to `dtype`:
  * a int8 [m, k] (rows lda bytes apart, one scale per token), wt int8 [n, k] (K-contiguous, rows ldw
- * apart, one scale per channel), as rmlk_hip_quantize_rows leaves both. The integer sums are exact.
+ * apart, one scale per channel), as rmlk_hip_quantize_rows leaves both. The integer sums are exact, the
+ * scales and the residual follow in float, from left to right.
  * residual (NULL: none) has rows ldr elements apart (0: one row for all, i.e. a bias) and may be c.
  * lda and ldw are multiples of 16 and at least k rounded up to 16, a and wt 16-byte aligned
- * (RMLK_ERR_UNSUPPORTED otherwise); what the bytes k .. of a row hold does not matter. k < 131072
- * (larger sums could leave 32 bits: RMLK_ERR_TOO_LARGE). The workspace holds
+ * (RMLK_ERR_UNSUPPORTED otherwise); what the bytes k .. of a row hold does not matter, but they are
+ * read up to the next 16, in the last row too. k < 131072 (larger sums could leave 32 bits), lda and
+ * ldw < 2^23: RMLK_ERR_TOO_LARGE beyond. The workspace holds
  * rmlk_hip_matmul_int8_workspace_size bytes (0 for most sizes), 16-byte aligned; its contents on
  * entry do not matter and it belongs to the call until its kernels have run. */
 size_t rmlk_hip_matmul_int8_workspace_size(int64_t m, int64_t n, int64_t k);
@@ -689,7 +692,10 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
  * re-rounded to a larger scale any number of times and stays within one (final) step of what was
  * appended: s/2 + s/4 + .. < s. page_size is 16, 32, 64 or 128, head_dim 64 or 128. V lies
  * transposed: the attention reads sixteen tokens of one head dim at a time. All arrays 16-byte
- * aligned. The caller owns them; a page needs no initialisation before its first append. */
+ * aligned. The caller owns them; a page needs no initialisation before its first append. There is at
+ * least one page, and fewer than 2^31; at most 65535 KV heads, as many heads of q, as many sequences in
+ * a call; fewer than 2^30 rows (times heads, for the attention) and tokens of a sequence
+ * (RMLK_ERR_TOO_LARGE beyond). */
 typedef struct rmlk_paged_cache {
     int64_t pages;          /* pages the arrays hold */
     int32_t page_size;
@@ -723,13 +729,14 @@ typedef struct rmlk_paged_batch {
 /* Appends the new tokens: k and v [rows, kv_heads, head_dim] (rows k_stride / v_stride elements apart),
  * k rotated like rmlk_hip_rotary with row t of the tables cos and sin, float [positions, head_dim], t the
  * token's position in its sequence (both NULL: k as it is; a token at a position >= positions is
- * skipped and reported, as is a sequence of fewer tokens than rows). A block's scale becomes the smallest power of two s with |x| <= 127 s for everything
- * appended to it, at least 2^-126; an append that starts at slot 0 of a page starts its blocks anew,
- * whatever they held. Rounding to nearest even, decided as in exact arithmetic. A NaN or an infinity
- * among a block's new values makes its scale NaN until the block is started anew, and the attention of
- * every query that sees a token of the block NaN. q (NULL: none), [rows, heads, head_dim], is rotated
- * alike into the dense q_out (may be q). A page that receives tokens belongs to one sequence of the
- * call. 16-byte aligned rows, heads a multiple of kv_heads; RMLK_ERR_UNSUPPORTED otherwise. */
+ * skipped and reported, as is a sequence of fewer tokens than rows). A block's scale becomes the
+ * smallest power of two s with |x| <= 127 s for everything appended to it, at least 2^-126; an append
+ * that starts at slot 0 of a page starts its blocks anew, whatever they held. Rounding to nearest even,
+ * decided as in exact arithmetic. A NaN or an infinity among a block's new values makes its scale NaN
+ * until the block is started anew, and the attention of every query that sees a token of the block NaN.
+ * q (NULL: none), [rows, heads, head_dim], is rotated alike into the dense q_out (may be q where that is
+ * dense). A page that receives tokens belongs to one sequence of the call, which has it once in its
+ * table. 16-byte aligned rows (RMLK_ERR_UNSUPPORTED otherwise), heads a multiple of kv_heads. */
 int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_paged_cache *cache,
                               const rmlk_paged_batch *batch, const void *k, int64_t k_stride,
                               const void *v, int64_t v_stride, const float *cos, const float *sin,
@@ -743,6 +750,7 @@ int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_pa
  * tokens) gives zeros. q has rows q_stride elements apart, out is dense [rows, heads, head_dim]; q is read
  * as one (16-bit types) or two half values (float, 22 significant bits relative to the row's largest)
  * and the cached integers exactly; scales that are no powers of two are rounded to 11 bits in V. The
+ * result does not overlap q, and the cache is not appended to meanwhile. The
  * workspace holds rmlk_hip_paged_attention_workspace_size bytes, 16-byte aligned (0 where the keys
  * are not split over blocks); its contents on entry do not matter, and it belongs to the call until its
  * kernels have run. */

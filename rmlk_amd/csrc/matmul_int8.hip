@@ -378,17 +378,21 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         });
     }
 
-    // The sums go through LDS, 32 rows of a wavefront's tile at a time, so that a lane has eight neighbouring
-    // outputs of a row: whole 16-byte accesses to c and the residual (an output per lane, 2 bytes each,
-    // took 150 us of a 417 us product of 4096 x 8192 x 8192 with a residual).
+    // The sums go through LDS, 32 rows of a wavefront's tile at a time, so that a lane has eight outputs of a row as
+    // 16-byte units of c and the residual (an output per lane, 2 bytes each, took 150 us of a 417 us product of
+    // 4096 x 8192 x 8192 with a residual). Units of neighbouring lanes are neighbours: a lane's two units of
+    // floats lie half a tile apart (next to each other, every store touched twice the lines: 509 x 8192 x 2048 took
+    // 17.3 us, and takes 15.9).
     __syncthreads();
     constexpr int kCols = 32 * TN, kPad = kCols + 4, kLanesPerRow = kCols / 8, kRowsPerTrip = kWave / kLanesPerRow;
     constexpr int kTrips = 32 / kRowsPerTrip;
     int32_t *mine = reinterpret_cast<int32_t *>(smem) + wave * 32 * kPad;
-    const int col = n0 + wn * kCols + lane % kLanesPerRow * 8;
+    constexpr int kApart = sizeof(T) == 4 ? kCols / 2 : 4;       // from a lane's first four columns to its other four
+    const int in_tile = lane % kLanesPerRow * (sizeof(T) == 4 ? 4 : 8), col = n0 + wn * kCols + in_tile;
+    auto col_of = [&](int e) { return col + e / 4 * kApart + e % 4; };
     float sw[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sw[e] = g.w_scale[min(col + e, g.n - 1)];
+    for (int e = 0; e < 8; ++e) sw[e] = g.w_scale[min(col_of(e), g.n - 1)];
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         T res[kTrips][8];
@@ -399,8 +403,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                 const int row = min(row0 + q * kRowsPerTrip, g.m - 1);
 #pragma unroll
                 for (size_t u = 0; u < sizeof(T) / 2; ++u)
-                    reinterpret_cast<u32x4 *>(res[q])[u] =
-                        reinterpret_cast<const u32x4 *>(g.residual + row * g.ldr + col)[u];
+                    if (const int at = col_of(4 * u); at < g.n)
+                        reinterpret_cast<u32x4 *>(res[q])[u] = *reinterpret_cast<const u32x4 *>(g.residual + row * g.ldr + at);
             }
         }
 #pragma unroll
@@ -413,14 +417,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
         for (int q = 0; q < kTrips; ++q) {
             const int row = row0 + q * kRowsPerTrip;
             int32_t sum[8];
-            const int32_t *from = mine + (lane / kLanesPerRow + q * kRowsPerTrip) * kPad + lane % kLanesPerRow * 8;
+            const int32_t *from = mine + (lane / kLanesPerRow + q * kRowsPerTrip) * kPad + in_tile;
             *reinterpret_cast<u32x4 *>(sum) = *reinterpret_cast<const u32x4 *>(from);
-            *reinterpret_cast<u32x4 *>(sum + 4) = *reinterpret_cast<const u32x4 *>(from + 4);
+            *reinterpret_cast<u32x4 *>(sum + 4) = *reinterpret_cast<const u32x4 *>(from + kApart);
             if (row >= g.m || col >= g.n) continue;
             if (g.sums) {
                 int32_t *to = g.sums + (static_cast<int64_t>(blockIdx.y) * g.m + row) * ((g.n + 7) & ~7) + col;
                 *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<u32x4 *>(sum);
-                *reinterpret_cast<u32x4 *>(to + 4) = *reinterpret_cast<u32x4 *>(sum + 4);
+                if (col + kApart < g.n) *reinterpret_cast<u32x4 *>(to + kApart) = *reinterpret_cast<u32x4 *>(sum + 4);
                 continue;
             }
             const float sa = g.a_scale[row];
@@ -434,9 +438,11 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                 }
 #pragma unroll
                 for (size_t u = 0; u < sizeof(T) / 2; ++u)
-                    reinterpret_cast<u32x4 *>(g.c + row * g.ldc + col)[u] = reinterpret_cast<u32x4 *>(out)[u];
+                    if (const int at = col_of(4 * u); at < g.n)
+                        *reinterpret_cast<u32x4 *>(g.c + row * g.ldc + at) = reinterpret_cast<u32x4 *>(out)[u];
             } else {
-                for (int e = 0; e < 8 && col + e < g.n; ++e) store_scaled(g, row, col + e, sum[e], sa, sw[e]);
+                for (int e = 0; e < 8; ++e)
+                    if (col_of(e) < g.n) store_scaled(g, row, col_of(e), sum[e], sa, sw[e]);
             }
         }
         __builtin_amdgcn_wave_barrier();
