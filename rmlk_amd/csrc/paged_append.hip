@@ -87,7 +87,8 @@ __device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
 #pragma unroll
-    for (size_t u = 0; u < sizeof(T) / 2; ++u) reinterpret_cast<u32x4 *>(to)[u] = reinterpret_cast<const u32x4 *>(v)[u];
+    for (size_t u = 0; u < sizeof(T) / 2; ++u)
+        __builtin_nontemporal_store(reinterpret_cast<const u32x4 *>(v)[u], reinterpret_cast<u32x4 *>(to) + u);
 }
 
 // The same for a 16-bit result, in float: the rounding error of one product is carried along, so that nothing is
@@ -111,8 +112,9 @@ __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[
             lo[i] = static_cast<T>(turn ? two_products(a[i], t.c0[i], -b[i], t.s0[i]) : a[i]);
             hi[i] = static_cast<T>(turn ? two_products(b[i], t.c1[i], a[i], t.s1[i]) : b[i]);
         }
-        *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<const u32x4 *>(lo);
-        *reinterpret_cast<u32x4 *>(to + half) = *reinterpret_cast<const u32x4 *>(hi);
+        // (streaming: no lines left to write back when the kernel ends)
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(lo), reinterpret_cast<u32x4 *>(to));
+        __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(hi), reinterpret_cast<u32x4 *>(to + half));
     }
 }
 

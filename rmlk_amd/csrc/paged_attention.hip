@@ -333,12 +333,12 @@ __device__ __forceinline__ int largest_step(float v_scale, bool odd) {
 template <typename T>
 __device__ __forceinline__ void store_four(T *to, const f32x4 &o) {
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<f32x4 *>(to) = o;
+        __builtin_nontemporal_store(o, reinterpret_cast<f32x4 *>(to));
     } else {
         T v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(o[e]);
-        *reinterpret_cast<u32x2 *>(to) = *reinterpret_cast<u32x2 *>(v);
+        __builtin_nontemporal_store(*reinterpret_cast<u32x2 *>(v), reinterpret_cast<u32x2 *>(to));
     }
 }
 
