@@ -50,7 +50,8 @@ __device__ __forceinline__ u32x4 clear_tail(u32x4 v, int valid) {
 // 16 channels x 16 * MT rows per block, v_mfma_i32_16x16x64_i8 with the channels as its rows: lane (l % 16,
 // l / 16) holds 16 consecutive bytes of channel l % 16, and of row l % 16 of a, straight from memory. A
 // wavefront takes every WAVES-th run of 256 bytes of K. Bytes of a behind k are cleared, so what the
-// weights hold there does not matter; units behind k are read from the row's start instead.
+// weights hold there does not matter; units behind k are read from the row's start instead. One row, 2048 channels,
+// K = 2048 (4.2 MB): 3.7 us, a launch and two trips to memory.
 template <typename T, int MT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave) void int8_few_rows_kernel(Int8Args<T> g) {
     __shared__ int32_t parts[WAVES][MT][kWave][4];
@@ -174,8 +175,12 @@ __global__ __launch_bounds__(kWideWaves *kWave) void int8_wide_kernel(Int8Args<T
 // step s + STAGES - 1 is requested in the first quarter of step s into the one read in step s - 1 (loads
 // complete in order: vmcnt tells when the next stage is there); one barrier per K step, in its last
 // quarter, behind which the first fragments of the next step are read. LDS reads and direct loads are
-// dealt out between the MFMAs. Rows behind m and n are read from the last
-// row and not stored.
+// dealt out between the MFMAs. Rows behind m and n are read from the last row and not stored.
+// 4096 x 8192 x 8192 in tiles of 256 x 256: 250 us, 2200 TOP/s, where the library's product reaches 2430 and the
+// matrix pipes are busy half of the cycles (a higher share lowers the clock). 509 x 8192 x 2048 in 256 tiles of
+// 128 x 128: 13.4 us; a K step takes 0.58 us, the time in which the L2s give a compute unit its 32 KB (14.5
+// TB/s in all), launch and first step 3.3 us, the stores 2 us. Measured and dropped there: 2 x 2
+// wavefronts (17.8 us at the time of 17.3), 64 x 128 tiles, two blocks per compute unit (20.3 us), two stages (23.2).
 template <typename T, int TM, int TN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, CHUNKS = 4;
@@ -382,7 +387,12 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     // 16-byte units of c and the residual (an output per lane, 2 bytes each, took 150 us of a 417 us product of
     // 4096 x 8192 x 8192 with a residual). Units of neighbouring lanes are neighbours: a lane's two units of
     // floats lie half a tile apart (next to each other, every store touched twice the lines: 509 x 8192 x 2048 took
-    // 17.3 us, then 16.0), and stores are streaming (no lines left to write back when the kernel ends: 14.1 us).
+    // 17.3 us, then 16.0). In the tiles of 128 columns stores are streaming: the kernel leaves no lines to write back
+    // when it ends (the same product 13.4 us; a layer of two products and the quantisation of their rows, 512 x 2048 x
+    // 8192 floats, 49.7 us against 51.1). The large results of the largest tiles have been written back by then, and
+    // are found closer by what reads them next (the same layer at 2048 rows: 113 us streamed, 107 us not), as are the
+    // few rows of the smallest ones (32 rows: 30.8 and 30.4 us).
+    constexpr bool kStreaming = BN == 128;
     __syncthreads();
     constexpr int kCols = 32 * TN, kPad = kCols + 4, kLanesPerRow = kCols / 8, kRowsPerTrip = kWave / kLanesPerRow;
     constexpr int kTrips = 32 / kRowsPerTrip;
@@ -438,9 +448,11 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                 }
 #pragma unroll
                 for (size_t u = 0; u < sizeof(T) / 2; ++u)
-                    if (const int at = col_of(4 * u); at < g.n)
-                        __builtin_nontemporal_store(reinterpret_cast<u32x4 *>(out)[u],
-                                                    reinterpret_cast<u32x4 *>(g.c + row * g.ldc + at));
+                    if (const int at = col_of(4 * u); at < g.n) {
+                        u32x4 *to = reinterpret_cast<u32x4 *>(g.c + row * g.ldc + at);
+                        if constexpr (kStreaming) __builtin_nontemporal_store(reinterpret_cast<u32x4 *>(out)[u], to);
+                        else *to = reinterpret_cast<u32x4 *>(out)[u];
+                    }
             } else {
                 for (int e = 0; e < 8; ++e)
                     if (col_of(e) < g.n) store_scaled(g, row, col_of(e), sum[e], sa, sw[e]);

@@ -81,14 +81,20 @@ __device__ __forceinline__ void rotate_eight(const float (&a)[8], const float (&
     }
 }
 
-template <typename T>
+// (STREAMING: past the caches, whose lines would have to be written back when the kernel ends)
+template <bool STREAMING>
+__device__ __forceinline__ void store_unit(void *to, u32x4 v) {
+    if constexpr (STREAMING) __builtin_nontemporal_store(v, static_cast<u32x4 *>(to));
+    else *static_cast<u32x4 *>(to) = v;
+}
+template <bool STREAMING, typename T>
 __device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
     T v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
 #pragma unroll
     for (size_t u = 0; u < sizeof(T) / 2; ++u)
-        __builtin_nontemporal_store(reinterpret_cast<const u32x4 *>(v)[u], reinterpret_cast<u32x4 *>(to) + u);
+        store_unit<STREAMING>(reinterpret_cast<u32x4 *>(to) + u, reinterpret_cast<const u32x4 *>(v)[u]);
 }
 
 // The same for a 16-bit result, in float: the rounding error of one product is carried along, so that nothing is
@@ -97,14 +103,14 @@ __device__ __forceinline__ float two_products(float x, float c, float y, float s
     const float p = y * s, rest = fmaf(y, s, -p);
     return fmaf(x, c, p) + (fabsf(p) < INFINITY ? rest : 0.f);
 }
-template <typename T>
+template <bool STREAMING, typename T>
 __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[8], const float (&b)[8], const Turn &t,
                                               bool turn) {
     if constexpr (sizeof(T) == 4) {
         double lo[8], hi[8];
         rotate_eight(a, b, t, turn, lo, hi);
-        store_eight(to, lo);
-        store_eight(to + half, hi);
+        store_eight<STREAMING>(to, lo);
+        store_eight<STREAMING>(to + half, hi);
     } else {
         T lo[8], hi[8];
 #pragma unroll
@@ -112,9 +118,8 @@ __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[
             lo[i] = static_cast<T>(turn ? two_products(a[i], t.c0[i], -b[i], t.s0[i]) : a[i]);
             hi[i] = static_cast<T>(turn ? two_products(b[i], t.c1[i], a[i], t.s1[i]) : b[i]);
         }
-        // (streaming: no lines left to write back when the kernel ends)
-        __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(lo), reinterpret_cast<u32x4 *>(to));
-        __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(hi), reinterpret_cast<u32x4 *>(to + half));
+        store_unit<STREAMING>(to, *reinterpret_cast<const u32x4 *>(lo));
+        store_unit<STREAMING>(to + half, *reinterpret_cast<const u32x4 *>(hi));
     }
 }
 
@@ -123,6 +128,13 @@ __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[
 // agree on the two largest magnitudes and write: one trip over the values. V is turned in LDS when more
 // than a few tokens come, so that the runs of new slots of a dim go out as whole words. The other blocks
 // rotate q.
+// Single tokens are a chain of trips to memory (the sequence, its page, values and scales): 64 of them, 8 KV heads
+// of 64 dims, 4.9 us. Prompts are bound by the bytes and by that chain in about equal parts: 2275 tokens of 8
+// sequences in bfloat16, 8 KV heads of 128 dims and 32 heads of q (53.6 MB) take 18.1 us, 13 us without q.
+// Measured and dropped: K and V in blocks of their own (20.8 became 26 us), units of 4 + 4 dims (25 us), q by
+// one or four heads per thread (1.1 us more; 2.2 us more with single tokens). Queries of 16-bit types turned in
+// double took 22.5 us when float took 20.8, plain stores of them 20.8 where streaming ones take 18.1 (with the
+// attention that reads them behind, 100 us either way; the queries of single tokens are stored as usual).
 template <typename T, int D, int THREADS, int PK>
 __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(AppendArgs<T> g) {
     constexpr int kUnitsK = D / 16, kUnitsV = D / 8;              // units of a token
@@ -158,7 +170,8 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
             if (g.cos) load_turn<D>(turn, g.cos, g.sin, pos, d);
 #pragma unroll
             for (int i = 0; i < kHeads; ++i)
-                if (h0 + i < g.heads) store_rotated(to + (h0 + i) * D, D / 2, x[i][0], x[i][1], turn, g.cos != nullptr);
+                if (h0 + i < g.heads)
+                    store_rotated<(THREADS > kWave)>(to + (h0 + i) * D, D / 2, x[i][0], x[i][1], turn, g.cos != nullptr);
         }
         return;
     }

@@ -418,7 +418,9 @@ __device__ __forceinline__ bool find_place(const AttendArgs<T> &g, int tile_rows
 }
 
 // Few rows (16 * NT of them): the wavefronts of a block deal the tiles of keys out among themselves, everything
-// in registers.
+// in registers. Bound by the cache's bytes: 64 single tokens behind 100 .. 16384 keys (8 KV heads of 128 dims, 415
+// MB) take 91 us with the join, 4.5 TB/s, where a large copy reaches 5.1. A single token behind 640 keys takes
+// 7.5 us, a chain of trips to memory (the sequence, its pages, three tiles per wavefront, the wavefronts' meeting).
 template <typename T, int D, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<T> g) {
     constexpr int DT = D / 16, KC = D / 64, R = 16 * NT, kPad = D + 4;
@@ -546,7 +548,15 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
 // Many rows: four wavefronts of 16 * NT rows each walk the same tiles of keys. A wavefront fetches and widens a
 // quarter of a tile and leaves it in LDS as the MFMA operands it is (64 lanes x 16 bytes each, read back as
 // they were written: no bank conflicts); two buffers, one barrier per tile. What widening costs, and the
-// trips to the caches, are shared by the block's rows.
+// trips to the caches, are shared by the block's rows. Bound by the issue of instructions: beside the 64 MFMAs of
+// a tile (D = 128, 16-bit types) a wavefront has some 270 vector instructions (32 exponentials and as many
+// arguments and maxima, the widening, addresses), and only a part of them runs under MFMAs: with two wavefronts per
+// SIMD, sixteen v_mfma_f32_16x16x32_f16 each take 541 cycles alone, 578, 595, 713 and 825 with one to four
+// multiply-adds behind every one of them, 566 with an exponential. So the scores of the next tile are computed beside
+// the weights of this one (a prompt of 8192 tokens, 32 heads of 128 dims: 627 us without, 585 us so, 940
+// TFLOP/s of the causal half), the largest score is looked for before the factors are applied, and an address is
+// one wide multiply. Measured and dropped: wavefront priorities (592 us), orders of MFMAs and vector instructions
+// given to the compiler (no faster), branches around the last fetch (the registers they hold).
 constexpr int kManyWaves = 4;
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(AttendArgs<T> g) {
@@ -774,9 +784,11 @@ Plan plan_for(const PagedArgs &c, int32_t dtype, int head_dim, int64_t heads) {
     const int64_t blocks = p.pieces * c.kv_heads;
     // Splits of the keys. A part costs its rows a trip through memory, and the call a second kernel.
     // Many rows: as many as make two blocks per compute unit (they are resident together: 512 rows behind 8192
-    // keys, 8 KV heads of 128 dims, take 103 us in 4 splits = 512 blocks, 115 us in 8); in a ragged call, where
-    // most sequences do not reach the bounds, four times that (the six sequences of the benchmark: 142 us,
-    // 182 us with the former rule); prompts with little before them are not thinned out for being ragged.
+    // keys, 8 KV heads of 128 dims, take 94 us in 4 splits = 512 blocks, 104 us in 6, 105 in 8, 134 in 16; a
+    // prompt of 2048 tokens in one piece 58 us, in two 71); in a ragged call, where most sequences do not reach
+    // the bounds, four times that (six sequences of 1 .. 512 rows behind 512 .. 16384 keys: 132 us, 195 us without
+    // the factor, 131 us with twice, 145 us with eight times); prompts with little before them are not thinned out
+    // for being ragged.
     // Few rows: a block per compute unit, and pieces of 2048 keys beyond 4096, so that sequences of different
     // lengths even out (64 sequences of 100 .. 16384 keys: 91 us, in pieces of 4096 109 us, of 1024 97 us; 32
     // sequences of 4096 keys: 52 us in one piece, 57 us in two). Up to 1024 keys the second kernel costs more
