@@ -523,12 +523,19 @@ struct Plan {
 };
 Plan plan_for(int64_t m, int64_t n, int64_t k) {
     auto tiles = [&](int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); };
+    auto rounds = [&](int bm, int bn) { return (tiles(bm, bn) + kNumCU - 1) / kNumCU; };
     Plan p{kTile64, 1, static_cast<int32_t>(k)};
+    // Each rule with both sides measured, in us, floats:
+    //   few rows, else tiles of 64 x 64:  32 x 2048 x 4096 7.7, 10.0; 32 x 8192 x 2048 8.0, 7.0
+    //   256 x 256, else 128 x 128, by the rounds of tiles (one of the large ones takes as long as 3.1 to 3.5 of the
+    //   others):  2048 x 8192 x 2048 43, 49; 1792 rows 41, 46; 1536 rows 40, 38; 2304 rows 68, 59
+    //   128 x 128, else 64 x 128:  352 x 8192 x 2048 11.4, 12.9; 256 rows 11.0, 10.0
+    //   64 x 128, else 64 x 64:  100 x 16384 x 2048 13.2, 14.0; 128 x 8192 x 2048 9.5, 7.6
     if (m > 4 && m <= 32 && n >= 64 * kNumCU && k > 0 && k <= 4096) {
         p.route = kWide;
     } else if (m <= 16 || (m <= 32 && n * k <= (1 << 23))) {
         p.route = kFewRows;
-    } else if (m > 128 && tiles(256, 256) >= kNumCU * 3 / 4) {
+    } else if (m > 128 && 10 * rounds(256, 256) <= 3 * rounds(128, 128)) {
         p.route = kTile256;
     } else if (m > 64 && tiles(128, 128) >= kNumCU * 11 / 16) {
         p.route = kTile128;

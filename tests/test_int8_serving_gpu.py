@@ -199,6 +199,14 @@ def test_matmul_int8_types_and_residuals(device, kind, residual, m):
     _product_case(device, kind, m, 333, 200, residual, m + 1, lda=256)
 
 
+@pytest.mark.parametrize("kind,residual", [("f32", None), ("f16", "rows"), ("bf16", "bias"), ("f32", "rows")])
+def test_matmul_int8_many_tiles(device, kind, residual):
+    """Sizes that take the largest tiles, whole and ragged in every direction."""
+    _product_case(device, kind, 509, 32704, 384, residual, 71)
+    _product_case(device, kind, 511, 32697, 130, residual, 72)
+    _product_case(device, kind, 385, 32520, 48, residual, 73, lda=64)
+
+
 def test_matmul_int8_largest_sums(device):
     """k at its limit and every product at its largest: the sums stay inside 32 bits."""
     k = 131071
