@@ -27,7 +27,6 @@ struct Int8Args {
     int32_t tiles_m, tiles_n;
     int32_t *sums;       // K split over blocks: the integer sums [splits][m][n rounded up to 8]
     int32_t k_per_split;
-    int32_t wide;        // eight outputs (and residuals) of a row are whole 16-byte units
 };
 
 template <typename T>
@@ -181,6 +180,8 @@ __global__ __launch_bounds__(kWideWaves *kWave) void int8_wide_kernel(Int8Args<T
 // 128 x 128: 13.4 us; a K step takes 0.58 us, the time in which the L2s give a compute unit its 32 KB (14.5
 // TB/s in all), launch and first step 3.3 us, the stores 2 us. Measured and dropped there: 2 x 2
 // wavefronts (17.8 us at the time of 17.3), 64 x 128 tiles, two blocks per compute unit (20.3 us), two stages (23.2).
+// Rows of a and wt that start inside a cache line make every step's 128 bytes cross from the L2 as two lines:
+// 635 x 26100 x 3550 takes 124 us with a pitch of 3552, 95 us with one of 3584.
 template <typename T, int TM, int TN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 128, CHUNKS = 4;
@@ -387,12 +388,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     // 16-byte units of c and the residual (an output per lane, 2 bytes each, took 150 us of a 417 us product of
     // 4096 x 8192 x 8192 with a residual). Units of neighbouring lanes are neighbours: a lane's two units of
     // floats lie half a tile apart (next to each other, every store touched twice the lines: 509 x 8192 x 2048 took
-    // 17.3 us, then 16.0). In the tiles of 128 columns stores are streaming: the kernel leaves no lines to write back
+    // 17.3 us, then 16.0); units start at any element (2279 x 3228 x 120 halves 11.5 us, element by element where rows
+    // are no whole units 22.3). In the tiles of 128 columns stores are streaming: the kernel leaves no lines to write back
     // when it ends (the same product 13.4 us; a layer of two products and the quantisation of their rows, 512 x 2048 x
     // 8192 floats, 49.7 us against 51.1). The large results of the largest tiles have been written back by then, and
     // are found closer by what reads them next (the same layer at 2048 rows: 113 us streamed, 107 us not), as are the
     // few rows of the smallest ones (32 rows: 30.8 and 30.4 us).
     constexpr bool kStreaming = BN == 128;
+    constexpr int kUnit = 16 / sizeof(T);
     __syncthreads();
     constexpr int kCols = 32 * TN, kPad = kCols + 4, kLanesPerRow = kCols / 8, kRowsPerTrip = kWave / kLanesPerRow;
     constexpr int kTrips = 32 / kRowsPerTrip;
@@ -407,14 +410,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
     for (int i = 0; i < TM; ++i) {
         T res[kTrips][8];
         const int row0 = m0 + (wm * TM + i) * 32 + lane / kLanesPerRow;
-        if (g.wide && g.residual && !g.sums && col < g.n) {
+        if (g.residual && !g.sums && col < g.n) {
 #pragma unroll
             for (int q = 0; q < kTrips; ++q) {
                 const int row = min(row0 + q * kRowsPerTrip, g.m - 1);
 #pragma unroll
                 for (size_t u = 0; u < sizeof(T) / 2; ++u)
-                    if (const int at = col_of(4 * u); at < g.n)
-                        reinterpret_cast<u32x4 *>(res[q])[u] = *reinterpret_cast<const u32x4 *>(g.residual + row * g.ldr + at);
+                    if (const int at = col_of(4 * u); at + kUnit <= g.n)
+                        reinterpret_cast<u32x4 *>(res[q])[u] = load_unit(g.residual + row * g.ldr + at);
             }
         }
 #pragma unroll
@@ -438,24 +441,23 @@ __global__ __launch_bounds__(WM *WN *kWave) void int8_tiles_kernel(Int8Args<T> g
                 continue;
             }
             const float sa = g.a_scale[row];
-            if (g.wide) {
-                T out[8];
+            T out[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float v = static_cast<float>(sum[e]) * sa * sw[e];
-                    if (g.residual) v += to_float(res[q][e]);
-                    out[e] = static_cast<T>(v);
+            for (int e = 0; e < 8; ++e) {
+                float v = static_cast<float>(sum[e]) * sa * sw[e];
+                if (g.residual) v += to_float(res[q][e]);
+                out[e] = static_cast<T>(v);
+            }
+#pragma unroll
+            for (size_t u = 0; u < sizeof(T) / 2; ++u) {
+                const int at = col_of(4 * u);
+                if (at + kUnit <= g.n) {
+                    store_unit<kStreaming>(g.c + row * g.ldc + at, reinterpret_cast<u32x4 *>(out)[u]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kUnit; ++e)
+                        if (at + e < g.n) store_scaled(g, row, at + e, sum[u * kUnit + e], sa, sw[u * kUnit + e]);
                 }
-#pragma unroll
-                for (size_t u = 0; u < sizeof(T) / 2; ++u)
-                    if (const int at = col_of(4 * u); at < g.n) {
-                        u32x4 *to = reinterpret_cast<u32x4 *>(g.c + row * g.ldc + at);
-                        if constexpr (kStreaming) __builtin_nontemporal_store(reinterpret_cast<u32x4 *>(out)[u], to);
-                        else *to = reinterpret_cast<u32x4 *>(out)[u];
-                    }
-            } else {
-                for (int e = 0; e < 8; ++e)
-                    if (col_of(e) < g.n) store_scaled(g, row, col_of(e), sum[e], sa, sw[e]);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -624,9 +626,6 @@ int32_t rmlk_hip_matmul_int8(rmlk_stream_t stream, int32_t dtype, int64_t m, int
         g.m = static_cast<int32_t>(m);
         g.n = static_cast<int32_t>(n);
         g.k = static_cast<int32_t>(k);
-        constexpr int64_t unit = 16 / sizeof(T);
-        g.wide = n % 8 == 0 && ldc % unit == 0 && aligned16(c) &&
-                 (!residual || (ldr % unit == 0 && aligned16(residual)));
         return launch_int8(st, g, plan_for(m, n, k), workspace);
     });
 }

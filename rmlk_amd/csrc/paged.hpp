@@ -29,6 +29,22 @@ __device__ __forceinline__ void load_row(const T *p, float (&out)[N]) {
     for (int i = 0; i < N; ++i) out[i] = to_float(v[i]);
 }
 
+// 16 bytes at any element's address: the memory takes such accesses wherever they start.
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ u32x4 load_unit(const T *p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const u32x4_at4 *>(p);
+    else return *reinterpret_cast<const u32x4_at2 *>(p);
+}
+template <bool STREAMING = false, typename T>
+__device__ __forceinline__ void store_unit(T *p, u32x4 v) {
+    if constexpr (STREAMING && sizeof(T) == 4) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at4 *>(p));
+    else if constexpr (STREAMING) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at2 *>(p));
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4_at4 *>(p) = v;
+    else *reinterpret_cast<u32x4_at2 *>(p) = v;
+}
+
 inline bool is_activation(int32_t dtype) {
     return dtype == RMLK_FLOAT || dtype == RMLK_FLOAT16 || dtype == RMLK_BFLOAT16;
 }

@@ -82,11 +82,6 @@ __device__ __forceinline__ void rotate_eight(const float (&a)[8], const float (&
 }
 
 // (STREAMING: past the caches, whose lines would have to be written back when the kernel ends)
-template <bool STREAMING>
-__device__ __forceinline__ void store_unit(void *to, u32x4 v) {
-    if constexpr (STREAMING) __builtin_nontemporal_store(v, static_cast<u32x4 *>(to));
-    else *static_cast<u32x4 *>(to) = v;
-}
 template <bool STREAMING, typename T>
 __device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
     T v[8];
@@ -94,7 +89,7 @@ __device__ __forceinline__ void store_eight(T *to, const double (&x)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
 #pragma unroll
     for (size_t u = 0; u < sizeof(T) / 2; ++u)
-        store_unit<STREAMING>(reinterpret_cast<u32x4 *>(to) + u, reinterpret_cast<const u32x4 *>(v)[u]);
+        store_unit<STREAMING>(to + u * (16 / sizeof(T)), reinterpret_cast<const u32x4 *>(v)[u]);
 }
 
 // The same for a 16-bit result, in float: the rounding error of one product is carried along, so that nothing is

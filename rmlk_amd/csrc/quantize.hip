@@ -26,24 +26,26 @@ __device__ __forceinline__ T block_reduce(T v, T *lds, Op op) {
     return r;
 }
 
-// Eight values of a row from column c on, zeros behind its end. ALIGNED: the row starts at a 16-byte boundary.
-template <bool ALIGNED, typename T>
+// Eight values of a row from column c on, zeros behind its end. Rows start where their elements do: the memory takes
+// 16-byte accesses at any address (4118 rows of 2941 bfloat16 14.1 us, element by element 15.9; 1729 rows of 9254
+// floats with the norm 33 us, 131 us element by element and held in registers).
+template <typename T>
 __device__ __forceinline__ void load_eight(const T *row, int c, int cols, T (&out)[8]) {
-    if (ALIGNED && c + 8 <= cols) {
+    if (c + 8 <= cols) {
 #pragma unroll
         for (size_t u = 0; u < sizeof(T) / 2; ++u)
-            reinterpret_cast<u32x4 *>(out)[u] = reinterpret_cast<const u32x4 *>(row + c)[u];
+            reinterpret_cast<u32x4 *>(out)[u] = load_unit(row + c + u * (16 / sizeof(T)));
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[e] = c + e < cols ? row[c + e] : static_cast<T>(0.f);
     }
 }
-template <bool ALIGNED, typename T>
+template <typename T>
 __device__ __forceinline__ void store_eight(T *row, int c, int cols, const T (&v)[8]) {
-    if (ALIGNED && c + 8 <= cols) {
+    if (c + 8 <= cols) {
 #pragma unroll
         for (size_t u = 0; u < sizeof(T) / 2; ++u)
-            reinterpret_cast<u32x4 *>(row + c)[u] = reinterpret_cast<const u32x4 *>(v)[u];
+            store_unit(row + c + u * (16 / sizeof(T)), reinterpret_cast<const u32x4 *>(v)[u]);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -64,7 +66,7 @@ __device__ __forceinline__ uint64_t pack_eight(const int (&n)[8]) {
 // CH = 0: a row of any length, read twice (the second time from the caches). Bound by the memory: 4096 rows of 8192
 // floats, 168 MB, take 34.2 us = 4.9 TB/s, where a large copy reaches 5.1. (Streaming stores of q: 31.9 us, but what
 // reads q next then waits for the memory: with a product of q and its scales behind it 133 us against 112.)
-template <typename T, int THREADS, int CH, bool ALIGNED>
+template <typename T, int THREADS, int CH>
 __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T *__restrict__ xs, int64_t ldx, int64_t rows,
                                                                 int32_t cols, int8_t *__restrict__ qs, int64_t ldq,
                                                                 float *__restrict__ scale) {
@@ -82,12 +84,12 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T *__restr
         };
         if constexpr (CH > 0) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) load_eight<ALIGNED>(x, (i * THREADS + tid) * 8, cols, held[i]);
+            for (int i = 0; i < CH; ++i) load_eight(x, (i * THREADS + tid) * 8, cols, held[i]);
 #pragma unroll
             for (int i = 0; i < CH; ++i) magnitude(held[i]);
         } else {
             for (int c = tid * 8; c < cols; c += THREADS * 8) {
-                load_eight<ALIGNED>(x, c, cols, held[0]);
+                load_eight(x, c, cols, held[0]);
                 magnitude(held[0]);
             }
         }
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T *__restr
                 if (const int c = (i * THREADS + tid) * 8; c < padded) quantize(held[i], c);
         } else {
             for (int c = tid * 8; c < padded; c += THREADS * 8) {
-                load_eight<ALIGNED>(x, c, cols, held[0]);
+                load_eight(x, c, cols, held[0]);
                 quantize(held[0], c);
             }
         }
@@ -121,11 +123,11 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T *__restr
     }
 }
 
-// The same behind RMSNorm: y = x * f * gamma with f = 1 / sqrt(mean(x^2) + eps). A thread holds the exact
-// products x * gamma (48 bits) in double; their largest magnitude times f is the row's, and
+// The same behind RMSNorm: y = x * f * gamma with f = 1 / sqrt(mean(x^2) + eps). The products x * gamma are exact
+// in double (48 bits); their largest magnitude times f is the row's, and
 // y / scale = x * gamma * (f / scale). One row of 2048 floats with a sum takes 2.9 us: a launch, a trip to memory
 // and three reductions over the block.
-template <typename T, int THREADS, int CH, bool ALIGNED>
+template <typename T, int THREADS, int CH>
 __global__ __launch_bounds__(THREADS) void norm_quantize_kernel(const T *xs, const T *bs, const float *__restrict__ gamma,
                                                                 float eps, int64_t rows, int32_t cols, T *sums,
                                                                 int8_t *__restrict__ qs, int64_t ldq,
@@ -136,42 +138,39 @@ __global__ __launch_bounds__(THREADS) void norm_quantize_kernel(const T *xs, con
         const T *x = xs + row * cols, *b = bs ? bs + row * cols : nullptr;
         T *sum = bs ? sums + row * cols : nullptr;
         int8_t *q = qs + row * ldq;
-        double held[CH > 0 ? CH : 1][8], square = 0.0, top = 0.0, odd = 0.0;
-        // loads a unit, forms the sum where there is one, adds up squares, leaves the products in p
-        auto products = [&](int c, double (&p)[8], const T (&v)[8], const T (&w)[8], const float (&gm)[8]) {
-            T t[8];
+        T held[CH > 0 ? CH : 1][8];
+        float gm[CH > 0 ? CH : 1][8];
+        double square = 0.0, top = 0.0, odd = 0.0;
+        // forms the sum of a unit where there is one, adds up squares, finds the largest product with gamma
+        auto measure = [&](int c, T (&v)[8], const T (&w)[8], const float (&gm)[8]) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                t[e] = v[e];
-                if (b) t[e] = static_cast<T>(to_float(v[e]) + to_float(w[e]));
-                const double y = to_float(t[e]);
+                if (b) v[e] = static_cast<T>(to_float(v[e]) + to_float(w[e]));
+                const double y = to_float(v[e]), p = y * static_cast<double>(gm[e]);
                 square = fma(y, y, square);
-                p[e] = y * static_cast<double>(gm[e]);
-                top = fmax(top, fabs(p[e]));
-                odd = fma(p[e], 0.0, odd);       // NaN with the first product that is not finite
+                top = fmax(top, fabs(p));
+                odd = fma(p, 0.0, odd);       // NaN with the first product that is not finite
             }
-            if (b && c < cols) store_eight<ALIGNED>(sum, c, cols, t);
+            if (b && c < cols) store_eight(sum, c, cols, v);
         };
         if constexpr (CH > 0) {
-            T v[CH][8], w[CH][8];
-            float gm[CH][8];
+            T w[CH][8];
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const int c = (i * THREADS + tid) * 8;
-                load_eight<ALIGNED>(x, c, cols, v[i]);
-                if (b) load_eight<ALIGNED>(b, c, cols, w[i]);
-                load_eight<ALIGNED>(gamma, c, cols, gm[i]);
+                load_eight(x, c, cols, held[i]);
+                if (b) load_eight(b, c, cols, w[i]);
+                load_eight(gamma, c, cols, gm[i]);
             }
 #pragma unroll
-            for (int i = 0; i < CH; ++i) products((i * THREADS + tid) * 8, held[i], v[i], w[i], gm[i]);
+            for (int i = 0; i < CH; ++i) measure((i * THREADS + tid) * 8, held[i], w[i], gm[i]);
         } else {
             for (int c = tid * 8; c < cols; c += THREADS * 8) {
-                T v[8], w[8];
-                float gm[8];
-                load_eight<ALIGNED>(x, c, cols, v);
-                if (b) load_eight<ALIGNED>(b, c, cols, w);
-                load_eight<ALIGNED>(gamma, c, cols, gm);
-                products(c, held[0], v, w, gm);
+                T w[8];
+                load_eight(x, c, cols, held[0]);
+                if (b) load_eight(b, c, cols, w);
+                load_eight(gamma, c, cols, gm[0]);
+                measure(c, held[0], w, gm[0]);
             }
         }
         auto add = [](double a, double c) { return a + c; };
@@ -186,44 +185,48 @@ __global__ __launch_bounds__(THREADS) void norm_quantize_kernel(const T *xs, con
         const bool zero = bad || amax < static_cast<double>(kSmallest);
         const float s = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.f : s_of;
         const double to_step = zero ? 0.0 : f / static_cast<double>(s);
-        auto quantize = [&](const double (&p)[8], int c) {
+        auto quantize = [&](const T (&v)[8], const float (&gm)[8], int c) {
             int n[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) n[e] = zero ? 0 : min(127, max(-127, static_cast<int>(rint(p[e] * to_step))));
+            for (int e = 0; e < 8; ++e) {
+                const double p = static_cast<double>(to_float(v[e])) * static_cast<double>(gm[e]);
+                n[e] = zero ? 0 : min(127, max(-127, static_cast<int>(rint(p * to_step))));
+            }
             *reinterpret_cast<uint64_t *>(q + c) = pack_eight(n);
         };
         if constexpr (CH > 0) {
 #pragma unroll
             for (int i = 0; i < CH; ++i)
-                if (const int c = (i * THREADS + tid) * 8; c < padded) quantize(held[i], c);
+                if (const int c = (i * THREADS + tid) * 8; c < padded) quantize(held[i], gm[i], c);
         } else {
             for (int c = tid * 8; c < padded; c += THREADS * 8) {
-                T v[8];
-                float gm[8];
-                load_eight<ALIGNED>(b ? sum : x, c, cols, v);      // (every thread reads back what it wrote itself)
-                load_eight<ALIGNED>(gamma, c, cols, gm);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) held[0][e] = static_cast<double>(to_float(v[e])) * static_cast<double>(gm[e]);
-                quantize(held[0], c);
+                load_eight(b ? sum : x, c, cols, held[0]);      // (every thread reads back what it wrote itself)
+                load_eight(gamma, c, cols, gm[0]);
+                quantize(held[0], gm[0], c);
             }
         }
         if (tid == 0) scale[row] = s;
     }
 }
 
-// f(threads, units per thread) as constants: a wavefront for short rows, larger blocks for longer ones, rows of
-// up to 16384 values held in registers. MOST: units a thread may hold (the norm's take 40 registers each).
-template <int MOST, typename F>
+// f(threads, units per thread) as constants: a wavefront for short rows, larger blocks for longer ones. Rows of up
+// to 16384 values are held in registers, behind the norm, which has gamma and a second operand besides, of up to
+// 4096: longer ones are read twice by 512 threads (4096 rows of 8192 floats with a sum: 95 us; held by 256 threads
+// 120, by 1024 threads 102 us; read twice by 256 threads 100. One row: 5.2, 5.8, 4.9 and 6.0 us).
+template <bool NORM, typename F>
 int32_t with_row_shape(int32_t cols, F &&f) {
     using std::integral_constant;
     const int units = (cols + 15) / 16 * 2;
     if (units <= 64) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     if (units <= 256) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     if (units <= 512) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    constexpr int kFour = MOST >= 4 ? 256 : 512, kEight = MOST >= 8 ? 256 : 1024;
-    if (units <= 1024) return f(integral_constant<int, kFour>{}, integral_constant<int, 1024 / kFour>{});
-    if (units <= 2048) return f(integral_constant<int, kEight>{}, integral_constant<int, 2048 / kEight>{});
-    return f(integral_constant<int, 256>{}, integral_constant<int, 0>{});
+    if constexpr (NORM) {
+        return f(integral_constant<int, 512>{}, integral_constant<int, 0>{});
+    } else {
+        if (units <= 1024) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+        if (units <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+        return f(integral_constant<int, 256>{}, integral_constant<int, 0>{});
+    }
 }
 inline uint32_t row_blocks(int64_t rows) { return static_cast<uint32_t>(rows < (1 << 20) ? rows : (1 << 20)); }
 
@@ -252,11 +255,9 @@ int32_t rmlk_hip_quantize_rows(rmlk_stream_t stream, int32_t dtype, int64_t rows
     if (!x || !q || !scale) return RMLK_ERR_NULL_POINTER;
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
-        const bool aligned = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-        return with_row_shape<8>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
+        return with_row_shape<false>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
             constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
-            auto kern = aligned ? quantize_rows_kernel<T, THREADS, CH, true> : quantize_rows_kernel<T, THREADS, CH, false>;
-            kern<<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), ldx, rows, static_cast<int32_t>(cols),
+            quantize_rows_kernel<T, THREADS, CH><<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), ldx, rows, static_cast<int32_t>(cols),
                                                         static_cast<int8_t *>(q), ldq, scale);
             return launch_status();
         });
@@ -272,12 +273,9 @@ int32_t rmlk_hip_rmsnorm_quantize_rows(rmlk_stream_t stream, int32_t dtype, int6
     if (!x || !gamma || !q || !scale || (b == nullptr) != (sum_out == nullptr)) return RMLK_ERR_NULL_POINTER;
     return with_activation(dtype, [&](auto tag) {
         using T = decltype(tag);
-        const bool aligned = cols * sizeof(T) % 16 == 0 && cols % 4 == 0 && aligned16(x) && aligned16(b) &&
-                             aligned16(sum_out) && aligned16(gamma);
-        return with_row_shape<2>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
+        return with_row_shape<true>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
             constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
-            auto kern = aligned ? norm_quantize_kernel<T, THREADS, CH, true> : norm_quantize_kernel<T, THREADS, CH, false>;
-            kern<<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps,
+            norm_quantize_kernel<T, THREADS, CH><<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps,
                                                         rows, static_cast<int32_t>(cols), static_cast<T *>(sum_out),
                                                         static_cast<int8_t *>(q), ldq, scale);
             return launch_status();

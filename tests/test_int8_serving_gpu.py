@@ -149,6 +149,22 @@ def test_rmsnorm_quantize_rows_in_place_and_not_finite(device):
     _check_rows(q, scale, y, 96, False)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [4099, 8201, 16400])
+def test_rmsnorm_quantize_rows_long_odd_rows_in_place(device, kind, cols):
+    """Rows that start at odd addresses and are read twice, the sum over its first or its second operand."""
+    rng = np.random.default_rng(cols)
+    for over in (0, 1):
+        ops = [_dev(rng.standard_normal((3, cols)).astype(np.float32), device, TYPES[kind]) for _ in range(2)]
+        total = (ops[0].float() + ops[1].float()).to(TYPES[kind])
+        gamma = rng.uniform(0.5, 1.5, cols).astype(np.float32)
+        q = torch.full((3, _padded(cols)), 5, dtype=torch.int8, device=device)
+        scale = torch.zeros(3, device=device)
+        _k().rmsnorm_quantize_rows(ops[0], _dev(gamma, device), 1e-5, q, scale, add=ops[1], sum_out=ops[over])
+        assert torch.equal(ops[over], total)
+        _check_rows(q, scale, ref.rmsnorm(_f64(total), gamma, 1e-5), cols, False)
+
+
 # ---- int8 products --------------------------------------------------------------------------------
 
 def _product_case(device, kind, m, n, k, residual, seed, lda=None, values=127):
