@@ -257,8 +257,9 @@ int32_t rmlk_hip_quantize_rows(rmlk_stream_t stream, int32_t dtype, int64_t rows
         using T = decltype(tag);
         return with_row_shape<false>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
             constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
-            quantize_rows_kernel<T, THREADS, CH><<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), ldx, rows, static_cast<int32_t>(cols),
-                                                        static_cast<int8_t *>(q), ldq, scale);
+            quantize_rows_kernel<T, THREADS, CH>
+                <<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), ldx, rows, static_cast<int32_t>(cols),
+                                                       static_cast<int8_t *>(q), ldq, scale);
             return launch_status();
         });
     });
@@ -275,9 +276,9 @@ int32_t rmlk_hip_rmsnorm_quantize_rows(rmlk_stream_t stream, int32_t dtype, int6
         using T = decltype(tag);
         return with_row_shape<true>(static_cast<int32_t>(cols), [&](auto threads, auto units) {
             constexpr int THREADS = decltype(threads)::value, CH = decltype(units)::value;
-            norm_quantize_kernel<T, THREADS, CH><<<row_blocks(rows), THREADS, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps,
-                                                        rows, static_cast<int32_t>(cols), static_cast<T *>(sum_out),
-                                                        static_cast<int8_t *>(q), ldq, scale);
+            norm_quantize_kernel<T, THREADS, CH><<<row_blocks(rows), THREADS, 0, st>>>(
+                static_cast<const T *>(x), static_cast<const T *>(b), gamma, eps, rows, static_cast<int32_t>(cols),
+                static_cast<T *>(sum_out), static_cast<int8_t *>(q), ldq, scale);
             return launch_status();
         });
     });
