@@ -518,14 +518,19 @@ def gemv_kmajor_head_rows(x, wt, k: int, streams, first_cols, gamma=None, eps: f
 # ---- 8-bit serving: int8 rows and products, a paged int8 cache ----------------------------------------
 
 def _pitch(t, width: int) -> int:
-    """Elements from one row to the next of a tensor [rows, ...] whose rows hold `width` dense elements."""
+    """Elements from one row to the next of a tensor [rows, ...] whose rows hold `width` dense elements. Rows that
+    repeat or overlap (expanded tensors) are refused: the kernels read and write every row where it would lie by
+    itself."""
     dense = 1
     for d in range(t.dim() - 1, 0, -1):
         n = t.shape[d]
         assert n == 1 or t.stride(d) == dense, "the elements of a row must be dense"
         dense *= n
     assert dense == width, f"rows hold {dense} elements, {width} expected"
-    return max(t.stride(0), width) if t.shape[0] > 1 else width
+    if t.shape[0] <= 1:
+        return width
+    assert t.stride(0) >= width, "rows must not overlap"
+    return t.stride(0)
 
 
 def _pitch2(t) -> int:
@@ -533,7 +538,10 @@ def _pitch2(t) -> int:
     rows, cols = t.shape
     pitch, one = t.stride()
     assert one == 1 or cols == 1, "the elements of a row must be dense"
-    return pitch if rows > 1 and pitch > cols else cols
+    if rows <= 1:
+        return cols
+    assert pitch >= cols, "rows must not overlap"
+    return pitch
 
 
 def _raw_stream(*tensors) -> int:
@@ -587,8 +595,8 @@ def matmul_int8_workspace_size(m: int, n: int, k: int) -> int:
 
 
 def matmul_int8(a, a_scale, wt, w_scale, out, k: int, residual=None, workspace=None) -> None:
-    """out[m, n] = (a[:, :k] . wt[:, :k]^T) * a_scale[:, None] * w_scale[None, :] (+ residual: [m, n], or [n] for
-    a bias), a int8 [m, ld] and wt int8 [n, ld] as quantize_rows leaves them."""
+    """out[m, n] = (a[:, :k] . wt[:, :k]^T) * a_scale[:, None] * w_scale[None, :] (+ residual: [m, n], or [n] (also
+    expanded to [m, n]) for a bias), a int8 [m, ld] and wt int8 [n, ld] as quantize_rows leaves them."""
     m, n = out.shape
     stream = _raw_stream(a, a_scale, wt, w_scale, out, residual, workspace)
     assert a.dtype is torch.int8 and wt.dtype is torch.int8 and a.shape[0] == m and wt.shape[0] == n
@@ -600,7 +608,10 @@ def matmul_int8(a, a_scale, wt, w_scale, out, k: int, residual=None, workspace=N
         assert residual.dtype is out.dtype
         if residual.dim() == 2:
             assert residual.shape == out.shape
-            ldr = _pitch2(residual)
+            if m > 1 and residual.stride(0) == 0:      # one row for all
+                assert n == 1 or residual.stride(1) == 1, "the elements of a row must be dense"
+            else:
+                ldr = _pitch2(residual)
         else:
             assert residual.shape == (n,) and residual.is_contiguous()
     handle = lib()
