@@ -17,6 +17,14 @@
 // exactly (V, f the page's step relative to the largest one met, E, which scales the output at the
 // end). So pages with different steps mix in one MFMA. K's step goes to the scores.
 //
+// That holds while the steps lie close together: a wavefront's rows share E, and a row's outputs would vanish
+// beside the step of a page that it does not see, or sees with next to no weight. Where the steps turn out to
+// spread over more than 2^kSpread, the tiles are gone through once more: V is widened as it is and the steps go to
+// the weights, each row's products of weight and step relative to the largest of its own. Within the range a page's
+// tokens lose what lies below 2^(kSpread - 31) of the row's largest product, less than V's own rounding (2^-8) even
+// where 2^14 of them do. (A prompt of 2048 tokens, 32 heads of 64 dims, floats: 53 us, with a tenth of the pages 2^20
+// apart 115 us; 64 single tokens behind 100 .. 16384 keys 91 and 113 us.)
+//
 // A float query is the sum of two halves (hi + lo, 22 bits), scaled by a power of two so that its
 // largest element lies in [2^13, 2^14); a float weight likewise, exponentials being taken relative to
 // the maximum less 7 and allowed to grow to 2^15 before the reference point moves (rescaling is rare),
@@ -34,6 +42,7 @@ constexpr int kTileKeys = 64;
 constexpr float kBase = 7.f;          // log2 of the weight of a key that scores the reference maximum
 constexpr float kLeastFactor = 1.17549435e-38f;
 constexpr float kMostWeight = 15.f;   // log2 of the largest weight before the reference point moves
+constexpr int kSpread = 6;            // log2 of the largest ratio of V's steps that share a reference
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -227,6 +236,8 @@ struct Softmax {
     // score becomes -inf before it is scaled: factors are kept positive, and where a row sees none of the lane
     // group's tokens its factor is replaced, so that a step that is no number reaches only the rows that see the
     // block.
+    // WIDE: the outputs have a reference of their own.
+    template <bool WIDE = false>
     __device__ __forceinline__ void refer(const Rows<T, D, NT> &rows, Scores &sc, float (&c)[NT], float kc, int t0,
                                           bool masked, bool bad) {
         const int key = t0 + threadIdx.x % kWave / 16 * 16;
@@ -262,8 +273,10 @@ struct Softmax {
                 const float alpha = now == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - now);
                 ref[n] = now;
                 sum[n] *= alpha;
+                if constexpr (!WIDE) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
+                    for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
+                }
             }
         }
     }
@@ -306,6 +319,75 @@ struct Softmax {
                     acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
         }
     }
+    // What the outputs are relative to once steps lie far apart: 2^num of the products of weight and step, a row's
+    // own, moved like ref and by the same bound. num is a whole number, so that a step's exponent adds to it exactly.
+    typedef float Reference[NT];
+    __device__ __forceinline__ void clear(Reference &num) {
+        clear();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) num[n] = ref[n];
+    }
+    // One tile from beginning to end, V as integers; step: the step of the lane group's tokens.
+    template <typename KF, typename VF>
+    __device__ __forceinline__ void wide_tile(const Rows<T, D, NT> &rows, KF &&k_frag, VF &&v_frag, float kc, float step,
+                                              int t0, bool masked, bool bad, Reference &num) {
+        Scores sc;
+        float c[NT];
+        scores(rows, k_frag, sc);
+        refer<true>(rows, sc, c, kc, t0, masked, bad);
+        int e = -200;
+        float m = 0.f;
+        if (step != 0.f && fabsf(step) <= 3.402823466e38f && !bad) m = frexpf(step, &e);
+        const float exponent = static_cast<float>(e);
+        float top[NT];
+        bool beyond = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            top[n] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top[n] = fmaxf(top[n], sc[i / 4][n][i % 4]);
+            top[n] = fmaf(top[n], c[n], exponent);
+            beyond = top[n] - num[n] > kMostWeight || beyond;
+        }
+        if (__any(beyond)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float now = fmaxf(num[n], rintf(across_groups_max(top[n]) - kBase));
+                const float alpha = now == num[n] ? 1.f : __builtin_amdgcn_exp2f(num[n] - now);
+                num[n] = now;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d][n] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            Weights pf;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float from = exponent - num[n];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float s = sc[hh * 2 + i / 4][n][i % 4];
+                    sum[n] += __builtin_amdgcn_exp2f(fmaf(s, c[n], -ref[n]));
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s, c[n], from)) * m;
+                    const _Float16 hi = static_cast<_Float16>(w);
+                    pf[0][n][i] = hi;
+                    if constexpr (P == 2) pf[1][n][i] = static_cast<_Float16>(w - static_cast<float>(hi));
+                }
+            }
+            outputs(v_frag, hh, pf);
+        }
+    }
+    // The outputs relative to a power of two again, each row's own.
+    __device__ __forceinline__ void close_range(const Reference &num, int (&unit)[NT]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float whole = rintf(ref[n]), f = __builtin_amdgcn_exp2f(whole - ref[n]);
+            unit[n] = static_cast<int>(fmaxf(-1000.f, fminf(1000.f, num[n] - whole)));
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d][n] *= f;
+        }
+    }
     // One tile from beginning to end.
     template <typename KF, typename VF>
     __device__ __forceinline__ void tile(const Rows<T, D, NT> &rows, KF &&k_frag, VF &&v_frag, float kc, int t0,
@@ -323,12 +405,19 @@ struct Softmax {
     }
 };
 
-// log2 of the largest step of V among the four lane groups' pages; a step that is no number counts as none.
-__device__ __forceinline__ int largest_step(float v_scale, bool odd) {
-    int e = odd ? -127 : static_cast<int>((__float_as_uint(v_scale) >> 23) & 255u) - 127;
-    return max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
-               max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
-}
+// log2 of the largest and the least step of V met. A step that is no number counts as the least there is.
+struct Steps {
+    int most = -200, least = 200;
+    // the four lane groups' pages of a tile
+    __device__ __forceinline__ void take(float v_scale, bool odd) {
+        const int e = odd ? -127 : static_cast<int>((__float_as_uint(v_scale) >> 23) & 255u) - 127;
+        const int a = __builtin_amdgcn_readlane(e, 0), b = __builtin_amdgcn_readlane(e, 16);
+        const int c = __builtin_amdgcn_readlane(e, 32), d = __builtin_amdgcn_readlane(e, 48);
+        most = max(most, max(max(a, b), max(c, d)));
+        least = min(least, min(min(a, b), min(c, d)));
+    }
+    __device__ __forceinline__ bool far() const { return most - least > kSpread; }
+};
 
 template <typename T>
 __device__ __forceinline__ void store_four(T *to, const f32x4 &o) {
@@ -433,6 +522,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     rows.load(g, p.s, p.kv, p.r0, p.rows);
     Softmax<T, D, NT> soft;
     soft.clear();
+    Steps steps;
     int step_exp = -200;       // E: log2 of the largest step of V met so far
 
     const View<D> view(g, p.s, p.seq, p.kv);
@@ -461,10 +551,10 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     auto compute = [&](const Tile<D> &t, int t0) {
         // V's steps relative to the largest; a step that is no number marks the scores instead
         const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
-        const int e = largest_step(t.v_scale, odd);
-        if (e > step_exp) {
-            soft.rescale(ldexpf(1.f, step_exp - e));
-            step_exp = e;
+        steps.take(t.v_scale, odd);
+        if (steps.most > step_exp) {
+            soft.rescale(ldexpf(1.f, step_exp - steps.most));
+            step_exp = steps.most;
         }
         const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
         const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
@@ -502,11 +592,36 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
                 }
                 compute(now, t0);
                 t0 = t1;
-                return more;
+                return more && !steps.far();
             };
             if (!half_step(one, two)) break;
             if (!half_step(two, one)) break;
         }
+    }
+    // steps that lie too far apart: all over again
+    int unit[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) unit[n] = step_exp;
+    if (__builtin_expect(steps.far(), 0)) {
+        typename Softmax<T, D, NT>::Reference num;
+        soft.clear(num);
+        for (t0 = p.begin + wave * kTileKeys; t0 < p.end; t0 += kStride) {
+            Tile<D> t;
+            uint32_t pk, pv;
+            pages_of(t0, pk, pv);
+            fetch(t, t0, pk, pv);
+            const bool marked = !(fabsf(t.v_scale) <= 3.402823466e38f) && !t.bad;
+            soft.wide_tile(
+                rows,
+                [&](int j, int q) {
+                    const u32x4 raw = t.k[j][q / 2];
+                    return q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
+                },
+                [&](int d, int hh) { return widen(t.v[d][2 * hh], t.v[d][2 * hh + 1]); },
+                marked ? __uint_as_float(0x7fc00000u) : t.k_scale, t.v_scale, t0,
+                t0 + kTileKeys > p.least || __any(t.bad), t.bad, num);
+        }
+        soft.close_range(num, unit);
     }
 
     // a wavefront's own mean first (bounded by the largest |v|), then the mean of the means
@@ -520,7 +635,7 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
         for (int d = 0; d < DT; ++d) {
             f32x4 o = soft.acc[d][n] * inv;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], step_exp);
+            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], unit[n]);
             *reinterpret_cast<f32x4 *>(lds + (wave * R + n * 16 + col) * kPad + d * 16 + grp * 4) = o;
         }
     }
@@ -602,10 +717,10 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     // what every wavefront knows of a tile whose V is in LDS
     struct Ready {
         float kc;
-        int step_exp;
+        int step_exp;          // E: log2 of the largest step of V met so far, the same in all wavefronts
         bool bad;
     };
-    int step_exp = -200;       // E: log2 of the largest step of V met so far, the same in all wavefronts
+    Steps steps;
     constexpr int kKFrags = 4 * KH, kVFrags = 2 * DT;
     u32x4 *const k_lds = frags + lane, *const v_lds = frags + 2 * kKFrags * kWave + lane;
     auto widen_k = [&](const Raw &t, int buf) {
@@ -618,8 +733,8 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     };
     auto widen_v = [&](const Raw &t, int buf) {
         const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
-        step_exp = max(step_exp, largest_step(t.v_scale, odd));
-        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
+        steps.take(t.v_scale, odd);
+        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -steps.most));
         const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
         const h2 vf = {f1, f1}, vbias = {b1, b1};
         u32x4 *to = v_lds + buf * kVFrags * kWave;
@@ -629,10 +744,10 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
             for (int hh = 0; hh < 2; ++hh)
                 to[((wave * DW + d) * 2 + hh) * kWave] =
                     __builtin_bit_cast(u32x4, widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias));
-        return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, step_exp, t.bad};
+        return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, steps.most, t.bad};
     };
 
-    int my_exp = -200;
+    int my_exp = -200, unit[NT] = {};
     if (p.begin < p.end) {
         // K is one tile ahead of V: a tile's scores are computed beside the weights of the tile before it, so that
         // the matrix cores and the other units have work at the same time. (Past the last tile the scores are of
@@ -695,6 +810,33 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
 #pragma unroll
                 for (int n = 0; n < NT; ++n) sc[j][n] = next[j][n];
         }
+        // steps that lie too far apart: all over again, one tile after the other
+#pragma unroll
+        for (int n = 0; n < NT; ++n) unit[n] = my_exp;
+        if (__builtin_expect(steps.far(), 0)) {
+            typename Softmax<T, D, NT>::Reference num;
+            soft.clear(num);
+            for (int t0 = p.begin; t0 < p.end; t0 += kTileKeys) {
+                fetch_k(raw, t0, k_page(t0));
+                fetch_v(raw, t0, v_page(t0));
+                __syncthreads();      // everyone has read what the buffers hold
+                widen_k(raw, 0);
+#pragma unroll
+                for (int d = 0; d < DW; ++d)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        v_lds[((wave * DW + d) * 2 + hh) * kWave] =
+                            __builtin_bit_cast(u32x4, widen(raw.v[d][2 * hh], raw.v[d][2 * hh + 1]));
+                __syncthreads();
+                const bool marked = !(fabsf(raw.v_scale) <= 3.402823466e38f) && !raw.bad;
+                soft.wide_tile(
+                    rows, [&](int j, int q) { return __builtin_bit_cast(h8, k_lds[(j * KH + q) * kWave]); },
+                    [&](int d, int hh) { return __builtin_bit_cast(h8, v_lds[(d * 2 + hh) * kWave]); },
+                    marked ? __uint_as_float(0x7fc00000u) : raw.k_scale, raw.v_scale, t0,
+                    t0 + kTileKeys > my_least || __any(raw.bad), raw.bad, num);
+            }
+            soft.close_range(num, unit);
+        }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -707,7 +849,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
         for (int d = 0; d < DT; ++d) {
             f32x4 o = soft.acc[d][n] * inv;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], my_exp);
+            for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], unit[n]);
             out.put(d * 16 + grp * 4, o, soft.ref[n], total);
         }
     }
