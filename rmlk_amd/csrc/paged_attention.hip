@@ -19,7 +19,7 @@
 //
 // That holds while the steps lie close together: a wavefront's rows share E, and a row's outputs would vanish
 // beside the step of a page that it does not see, or sees with next to no weight. Where the steps turn out to
-// spread over more than 2^kSpread, the tiles are gone through once more: V is widened as it is and the steps go to
+// spread over more than 2^kSpread, or one is no power of two, the tiles are gone through once more: V is widened as it is and the steps go to
 // the weights, each row's products of weight and step relative to the largest of its own. Within the range a page's
 // tokens lose what lies below 2^(kSpread - 31) of the row's largest product, less than V's own rounding (2^-8) even
 // where 2^14 of them do. (A prompt of 2048 tokens, 32 heads of 64 dims, floats: 53 us, with a tenth of the pages 2^20
@@ -319,7 +319,7 @@ struct Softmax {
                     acc[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p][n], acc[d][n], 0, 0, 0);
         }
     }
-    // What the outputs are relative to once steps lie far apart: 2^num of the products of weight and step, a row's
+    // What the outputs are relative to where steps lie far apart: 2^num of the products of weight and step, a row's
     // own, moved like ref and by the same bound. num is a whole number, so that a step's exponent adds to it exactly.
     typedef float Reference[NT];
     __device__ __forceinline__ void clear(Reference &num) {
@@ -369,7 +369,10 @@ struct Softmax {
                 for (int i = 0; i < 8; ++i) {
                     const float s = sc[hh * 2 + i / 4][n][i % 4];
                     sum[n] += __builtin_amdgcn_exp2f(fmaf(s, c[n], -ref[n]));
-                    const float w = __builtin_amdgcn_exp2f(fmaf(s, c[n], from)) * m;
+                    float w = __builtin_amdgcn_exp2f(fmaf(s, c[n], from)) * m;
+                    // (the product as it is rounded to float: formed once more inside a multiplication that rounds to
+                    // half, a tie falls the other way, and the rest below belongs to another half)
+                    asm("" : "+v"(w));
                     const _Float16 hi = static_cast<_Float16>(w);
                     pf[0][n][i] = hi;
                     if constexpr (P == 2) pf[1][n][i] = static_cast<_Float16>(w - static_cast<float>(hi));
@@ -405,12 +408,15 @@ struct Softmax {
     }
 };
 
-// log2 of the largest and the least step of V met. A step that is no number counts as the least there is.
+// log2 of the largest and the least step of V met. A step that is no number counts as the least that appends leave, one
+// that is no power of two (a caller's own) lies apart from every other: widen_scaled is exact for powers of two only,
+// in its product as in its bias.
 struct Steps {
     int most = -200, least = 200;
     // the four lane groups' pages of a tile
     __device__ __forceinline__ void take(float v_scale, bool odd) {
-        const int e = odd ? -127 : static_cast<int>((__float_as_uint(v_scale) >> 23) & 255u) - 127;
+        const uint32_t bits = __float_as_uint(v_scale);
+        const int e = odd ? -127 : bits & 0x807fffffu ? -1000 : static_cast<int>(bits >> 23) - 127;
         const int a = __builtin_amdgcn_readlane(e, 0), b = __builtin_amdgcn_readlane(e, 16);
         const int c = __builtin_amdgcn_readlane(e, 32), d = __builtin_amdgcn_readlane(e, 48);
         most = max(most, max(max(a, b), max(c, d)));

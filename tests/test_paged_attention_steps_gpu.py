@@ -146,3 +146,34 @@ def test_marked_pages_among_far_steps(device):
         sees = length - new + np.arange(new) + 1
         bad = torch.isnan(out).any(dim=2).cpu().numpy()
         assert np.array_equal(bad[:, 2], sees > 48) and np.array_equal(bad[:, 3], sees > 48) and not bad[:, :2].any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,rep", [(1, 4), (8, 4), (60, 3)])
+def test_steps_that_are_no_powers_of_two(device, kind, dim, new, rep):
+    """Scales of the caller's own making; some pages of theirs beside some of powers of two, near and far."""
+    for steps in ([0.0131], [0.0156, 4 / 3], [0.25, 0.3], [0.5, 0.25, 0.125, 0.7], [1.9999999, 2.0 ** -30, 0.01]):
+        p = _paged(device, 2, 16, 2, dim, 240, 3, [steps, steps[::-1]])
+        _run(p, kind, [new, new], [new + 12, new + 170], rep)
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_odd_steps_of_zeros_and_of_constants(device, new):
+    """A V of zeros gives zeros, one of ones its step, whatever the step."""
+    for kind in TYPES:
+        for step in (0.0131, 0.0156, 4 / 3, 5e-3, 0.9999):
+            p = _paged(device, 1, 16, 1, 64, 120, 4, [[step]])
+            for value in (0, 1, -1):
+                p.ref.v[:] = value
+                p.dev.v.copy_(torch.from_numpy(p.ref.v))
+                out = _run(p, kind, [new], [new + 50], 2)
+                if value == 0:
+                    assert not out.any()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_steps_of_a_caller_that_are_subnormal_zero_or_negative(device, new):
+    for steps in ([3e-40], [1e-39, 2.0 ** -126], [0.0], [0.0, 0.5, 0.0], [-0.3, 0.3], [-0.5]):
+        p = _paged(device, 1, 16, 1, 64, 120, 8, [steps])
+        _run(p, "f32", [new], [new + 50], 2)
