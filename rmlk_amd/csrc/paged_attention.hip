@@ -437,6 +437,14 @@ __device__ __forceinline__ void store_four(T *to, const f32x4 &o) {
     }
 }
 
+// Means of means are formed with weights that add up to less than one: values next to the largest float stay inside
+// it. (A power of two: nothing is rounded.)
+__device__ __forceinline__ int unit_of(float total) {
+    int e;
+    frexpf(total, &e);
+    return total > 0.f && total < INFINITY ? e : 0;
+}
+
 // Where a row's outputs go: the result, or (more than one split) a part of it with its statistics.
 template <typename T, int D>
 struct Output {
@@ -653,15 +661,18 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w * R + row].x);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        float total = 0.f;
+        float total = 0.f, weight[WAVES];
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             const float2 st = stats[w * R + row];
-            const float weight = st.y == 0.f ? 0.f : st.y * __builtin_amdgcn_exp2f(st.x - top);
-            total += weight;
-            o += *reinterpret_cast<const f32x4 *>(lds + (w * R + row) * kPad + d) * weight;
+            weight[w] = st.y == 0.f ? 0.f : st.y * __builtin_amdgcn_exp2f(st.x - top);
+            total += weight[w];
         }
-        o *= total == 0.f ? 0.f : 1.f / total;
+        const int unit = unit_of(total);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            o += *reinterpret_cast<const f32x4 *>(lds + (w * R + row) * kPad + d) * ldexpf(weight[w], -unit);
+        o *= total == 0.f ? 0.f : 1.f / ldexpf(total, -unit);
         Output<T, D>(g, p.s, p.kv, p.r0 + row, p.split).put(d, o, top, total);
     }
 }
@@ -879,6 +890,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
     // groups of eight parts, their loads in flight together; the reference point moves between groups
     constexpr int kGroup = 8;
     float top = -INFINITY, total = 0.f;
+    int unit = 0;        // of o
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < parts; i0 += kGroup) {
         float2 st[kGroup];
@@ -896,15 +908,19 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs<T> g) {
         const float alpha = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(top - now);
         top = now;
         total *= alpha;
-        o *= alpha;
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
-            const float weight = st[i].y == 0.f ? 0.f : st[i].y * __builtin_amdgcn_exp2f(st[i].x - top);
-            total += weight;
-            o += v[i] * weight;
+            st[i].y = st[i].y == 0.f ? 0.f : st[i].y * __builtin_amdgcn_exp2f(st[i].x - top);
+            total += st[i].y;
         }
+        const int was = unit;
+        unit = unit_of(total);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j] * alpha, was - unit);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) o += v[i] * ldexpf(st[i].y, -unit);
     }
-    store_four(g.out + at * D + d, o * (total == 0.f ? 0.f : 1.f / total));
+    store_four(g.out + at * D + d, o * (total == 0.f ? 0.f : 1.f / ldexpf(total, -unit)));
 }
 
 // How a call is cut: rows per block, tiles of rows, splits of the keys.

@@ -177,3 +177,27 @@ def test_steps_of_a_caller_that_are_subnormal_zero_or_negative(device, new):
     for steps in ([3e-40], [1e-39, 2.0 ** -126], [0.0], [0.0, 0.5, 0.0], [-0.3, 0.3], [-0.5]):
         p = _paged(device, 1, 16, 1, 64, 120, 8, [steps])
         _run(p, "f32", [new], [new + 50], 2)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_extreme_steps(device, kind, new):
+    """The smallest and the largest step a float has."""
+    p = _paged(device, 1, 16, 1, 64, 200, 6, [[2.0 ** -126, 2.0 ** -126, 2.0 ** 119, 2.0 ** -126]])
+    _run(p, kind, [new], [new], 2)
+    _run(p, kind, [new], [new + 60], 2)
+
+
+@pytest.mark.parametrize("new,length", [(1, 50), (1, 900), (3, 5000), (60, 200), (60, 3000)])
+def test_values_next_to_the_largest_float(device, new, length):
+    """Every value as large as a float can be: the results are means of them, in one piece, of wavefronts, of splits."""
+    p = _paged(device, 2, 16, 1, 64, length, 9, [[2.0 ** 121]])
+    p.ref.v[:] = np.where(p.ref.v < 0, -127, 127)
+    p.dev.v.copy_(torch.from_numpy(p.ref.v))
+    for scores in ([0], [5, -5, 3]):
+        for j, page in enumerate(p.table.reshape(-1)):
+            p.ref.k[page], p.ref.k_scale[page] = 0, 1.0
+            p.ref.k[page][..., 0] = scores[j % len(scores)]
+        p.dev.k.copy_(torch.from_numpy(p.ref.k))
+        p.dev.k_scale.copy_(torch.from_numpy(p.ref.k_scale))
+        _run(p, "f32", [new, new], [length, length - 7], 2, q=_query(2 * new, 2, 64))
