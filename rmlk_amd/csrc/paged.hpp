@@ -8,7 +8,7 @@ namespace rmlk {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Activation types: float, _Float16, __bf16. to_float is exact, from_float rounds to nearest even.
+// Activation types: float, _Float16, __bf16. to_float is exact; the casts back round to nearest even.
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;
 

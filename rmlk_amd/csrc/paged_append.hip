@@ -4,8 +4,9 @@
 // the new tokens' largest magnitude a, e has to satisfy a <= 127 * 2^e: with a = f * 2^x, f in [1/2, 1),
 // that is x - 7 for f <= 127/128 and x - 6 otherwise. A block that is continued keeps the larger of
 // this and the exponent it has; when it grows, the integers held already are shifted right with
-// rounding to nearest even. Rotation and quantisation are evaluated in double (two exact products and
-// one sum): a value next to the border between two integers falls the right way.
+// rounding to nearest even. Rotation and quantisation are evaluated in double, two exact products and their
+// sum rounded to odd: such a sum lies on a border (between two integers, or 127 * 2^e, numbers of few bits) only if
+// the real one does, and on the same side of it otherwise, so that every value falls the right way.
 #include <cmath>
 
 #include "paged.hpp"
@@ -71,6 +72,19 @@ __device__ __forceinline__ void load_turn(Turn &t, const float *cos, const float
     load_row(cos + pos * D + d + D / 2, t.c1);
     load_row(sin + pos * D + d + D / 2, t.s1);
 }
+// a + b rounded to 53 bits, towards the neighbour whose last bit is 1 where it is not exact (the error of the sum as in
+// Knuth's two-sum; rounding to odd as Boldo and Melquiond describe it). Sums that are not finite stay as they are.
+__device__ __forceinline__ double sum_to_odd(double a, double b) {
+    const double s = a + b, from_b = s - a, err = (a - (s - from_b)) + (b - from_b);
+    long long bits = __double_as_longlong(s);
+    const bool inexact = err > 0.0 || err < 0.0;
+    bits += inexact && !(bits & 1) ? ((err > 0.0) == (s > 0.0) ? 1 : -1) : 0;
+    return __longlong_as_double(bits);
+}
+// Zero for numbers of up to 9 bits, as the borders are.
+__device__ __forceinline__ uint32_t bits_behind_nine(double x) {
+    return static_cast<uint32_t>(__double2hiint(x) & 0xfff) | static_cast<uint32_t>(__double2loint(x));
+}
 __device__ __forceinline__ void rotate_eight(const float (&a)[8], const float (&b)[8], const Turn &t, bool turn,
                                              double (&lo)[8], double (&hi)[8]) {
 #pragma unroll
@@ -78,6 +92,16 @@ __device__ __forceinline__ void rotate_eight(const float (&a)[8], const float (&
         const double x = a[i], y = b[i];
         lo[i] = turn ? x * t.c0[i] + -y * t.s0[i] : x;
         hi[i] = turn ? y * t.c1[i] + x * t.s1[i] : y;
+    }
+}
+// The same with sums to odd.
+__device__ __forceinline__ void rotate_eight_to_odd(const float (&a)[8], const float (&b)[8], const Turn &t,
+                                                    double (&lo)[8], double (&hi)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double x = a[i], y = b[i];
+        lo[i] = sum_to_odd(x * t.c0[i], -y * t.s0[i]);
+        hi[i] = sum_to_odd(y * t.c1[i], x * t.s1[i]);
     }
 }
 
@@ -124,7 +148,7 @@ __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[
 // than a few tokens come, so that the runs of new slots of a dim go out as whole words. The other blocks
 // rotate q.
 // Single tokens are a chain of trips to memory (the sequence, its page, values and scales): 64 of them, 8 KV heads
-// of 64 dims, 4.9 us. Prompts are bound by the bytes and by that chain in about equal parts: 2275 tokens of 8
+// of 64 dims, 5.1 us. Prompts are bound by the bytes and by that chain in about equal parts: 2275 tokens of 8
 // sequences in bfloat16, 8 KV heads of 128 dims and 32 heads of q (53.6 MB) take 18.1 us, 13 us without q.
 // Measured and dropped: K and V in blocks of their own (20.8 became 26 us), units of 4 + 4 dims (25 us), q by
 // one or four heads per thread (1.1 us more; 2.2 us more with single tokens). Queries of 16-bit types turned in
@@ -220,6 +244,7 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
         if (t < tokens) load_row(g.v + (row0 + t) * g.v_stride + static_cast<int64_t>(head) * D + unit_v, v[i]);
     }
     double k_top = 0.0, odd = 0.0;
+    bool on_border = false;
     uint32_t v_bits = 0;
 #pragma unroll
     for (int i = 0; i < PK; ++i) {
@@ -232,6 +257,35 @@ __global__ __launch_bounds__(THREADS, PK < 4 ? 3 : 2) void paged_append_kernel(A
             Turn turn;
             if (g.cos) load_turn<D>(turn, g.cos, g.sin, pos0 + t, unit_k);
             rotate_eight(x[0], x[1], turn, g.cos != nullptr, k_lo[i], k_hi[i]);
+            uint32_t behind = ~0u, second = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                behind = min(behind, min(bits_behind_nine(k_lo[i][e]), bits_behind_nine(k_hi[i][e])));
+                second |= __float_as_uint(turn.s0[e]) | __float_as_uint(turn.s1[e]);
+            }
+            on_border = on_border || (behind == 0 && second << 1 != 0);     // (without a second product all is exact)
+        }
+    }
+    // A sum that rounding has not moved onto a border lies on the real one's side of all of them: to odd only where
+    // one is on a border now (for every sum, 64 single tokens take 5.6 us, so 5.1).
+    if (g.cos && __any(on_border)) {
+#pragma unroll
+        for (int i = 0; i < PK; ++i) {
+            const int t = i * kTokensK + tid / kUnitsK;
+            if (t < tokens) {
+                const T *from = g.k + (row0 + t) * g.k_stride + static_cast<int64_t>(head) * D + unit_k;
+                float x[2][8];
+                load_row(from, x[0]);
+                load_row(from + D / 2, x[1]);
+                Turn turn;
+                load_turn<D>(turn, g.cos, g.sin, pos0 + t, unit_k);
+                rotate_eight_to_odd(x[0], x[1], turn, k_lo[i], k_hi[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PK; ++i) {
+        if (i * kTokensK + tid / kUnitsK < tokens) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 k_top = fmax(k_top, fmax(fabs(k_lo[i][e]), fabs(k_hi[i][e])));
