@@ -750,11 +750,13 @@ int32_t rmlk_hip_paged_append(rmlk_stream_t stream, int32_t dtype, const rmlk_pa
  * tokens) gives zeros. q has rows q_stride elements apart, out is dense [rows, heads, head_dim]; q is read
  * as one (16-bit types) or two half values (float, 22 significant bits relative to the row's largest)
  * and the cached integers and scales exactly, whatever the scales of neighbouring pages; scales of V that
- * are no powers of two, or lie more than 2^6 apart, cost a second pass over the keys. K's scales are not
- * negative. The result does not overlap q, and the cache is not appended to meanwhile. The
- * workspace holds rmlk_hip_paged_attention_workspace_size bytes, 16-byte aligned (0 where the keys
- * are not split over blocks); its contents on entry do not matter, and it belongs to the call until its
- * kernels have run. */
+ * are no powers of two, or lie more than 2^6 apart, make a call slower. K's scales are not negative.
+ * The weights of the tokens are formed in float; with a float q they are multiplied with V as two halves
+ * (22 bits), with 16-bit types as one (rounded to 11 bits, the sum of the weights being that of the
+ * rounded ones, formed in float). The result does not overlap q, and the cache is not appended to
+ * meanwhile. The workspace holds rmlk_hip_paged_attention_workspace_size bytes, 16-byte aligned (0 where
+ * the keys are not split over blocks); its contents on entry do not matter, and it belongs to the call
+ * until its kernels have run. */
 size_t rmlk_hip_paged_attention_workspace_size(int32_t dtype, const rmlk_paged_cache *cache,
                                                const rmlk_paged_batch *batch, int64_t heads);
 int32_t rmlk_hip_paged_attention(rmlk_stream_t stream, int32_t dtype, const rmlk_paged_cache *cache,

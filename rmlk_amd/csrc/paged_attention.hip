@@ -14,16 +14,17 @@
 //
 // int8 -> half: a byte b with its sign bit flipped, u = b + 128, under the high byte 0x64 is the half
 // 1024 + u; one packed add of -1152 gives b (K), one packed fma (1024 + u) * f - 1152 f gives b * f
-// exactly (V, f the page's step relative to the largest one met, E, which scales the output at the
-// end). So pages with different steps mix in one MFMA. K's step goes to the scores.
+// exactly (V, f the page's step relative to the largest one of the block's keys, 2^E, which scales the output
+// at the end). So pages with different steps mix in one MFMA. K's step goes to the scores.
 //
 // That holds while the steps lie close together: a wavefront's rows share E, and a row's outputs would vanish
-// beside the step of a page that it does not see, or sees with next to no weight. Where the steps turn out to
-// spread over more than 2^kSpread, or one is no power of two, the tiles are gone through once more: V is widened as it is and the steps go to
-// the weights, each row's products of weight and step relative to the largest of its own. Within the range a page's
-// tokens lose what lies below 2^(kSpread - 31) of the row's largest product, less than V's own rounding (2^-8) even
-// where 2^14 of them do. (A prompt of 2048 tokens, 32 heads of 64 dims, floats: 53 us, with a tenth of the pages 2^20
-// apart 115 us; 64 single tokens behind 100 .. 16384 keys 91 and 113 us.)
+// beside the step of a page that it does not see, or sees with next to no weight. So the steps are looked over
+// first. Where they spread over more than 2^kSpread, or one is no power of two, V is widened as it is and the steps
+// go to the weights, each row's products of weight and step relative to the largest of its own (the wide loops).
+// Within the range a page's tokens lose what lies below 2^(kSpread - 31) of the row's largest product, less than V's
+// own rounding (2^-8) even where 2^14 of them do. (A prompt of 2048 tokens, 32 heads of 64 dims, floats: 51 us, with a
+// tenth of the pages 2^20 apart 79 us; 64 single tokens behind 100 .. 16384 keys 90 and 94 us. Looked over in the loops
+// instead, tile by tile, prompts of 64 dims took 4 % longer, and a cache of far steps a second pass.)
 //
 // A float query is the sum of two halves (hi + lo, 22 bits), scaled by a power of two so that its
 // largest element lies in [2^13, 2^14); a float weight likewise, exponentials being taken relative to
@@ -179,8 +180,9 @@ struct View {
         v += kv * size * D;
         pitch = heads * static_cast<uint32_t>(size * D);
     }
+    __device__ __forceinline__ int page_at(int token) const { return min(token >> shift, last_page); }
     __device__ __forceinline__ uint32_t page_of(int token) const {
-        return static_cast<uint32_t>(table[static_cast<uint32_t>(min(token >> shift, last_page))]);
+        return static_cast<uint32_t>(table[static_cast<uint32_t>(page_at(token))]);
     }
     __device__ __forceinline__ bool has(uint32_t page) const { return page < pages; }
     __device__ __forceinline__ const int8_t *at(const int8_t *base, uint32_t page, uint32_t offset) const {
@@ -204,12 +206,6 @@ struct Softmax {
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-    }
-    __device__ __forceinline__ void rescale(float f) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[d][n] *= f;
     }
     // S^T of a tile: k_frag(jj, h) gives K's operands.
     typedef f32x4 Scores[4][NT];
@@ -408,21 +404,42 @@ struct Softmax {
     }
 };
 
-// log2 of the largest and the least step of V met. A step that is no number counts as the least that appends leave, one
-// that is no power of two (a caller's own) lies apart from every other: widen_scaled is exact for powers of two only,
-// in its product as in its bias.
+// The steps of V of a block's keys. One that is no number does not count.
 struct Steps {
-    int most = -200, least = 200;
-    // the four lane groups' pages of a tile
-    __device__ __forceinline__ void take(float v_scale, bool odd) {
-        const uint32_t bits = __float_as_uint(v_scale);
-        const int e = odd ? -127 : bits & 0x807fffffu ? -1000 : static_cast<int>(bits >> 23) - 127;
-        const int a = __builtin_amdgcn_readlane(e, 0), b = __builtin_amdgcn_readlane(e, 16);
-        const int c = __builtin_amdgcn_readlane(e, 32), d = __builtin_amdgcn_readlane(e, 48);
-        most = max(most, max(max(a, b), max(c, d)));
-        least = min(least, min(min(a, b), min(c, d)));
+    int most = 0, least = 0x7f000000, others = 0;      // as bits: floats order like them
+    template <typename V>
+    __device__ __forceinline__ float step_of(const V &view, uint32_t page) const {
+        return view.v_scale[view.scale_at(view.has(page) ? page : 0)];
     }
-    __device__ __forceinline__ bool far() const { return most - least > kSpread; }
+    __device__ __forceinline__ void take(float step, bool counts) {
+        counts = counts && fabsf(step) <= 3.402823466e38f;
+        const int bits = __float_as_int(step);
+        most = counts ? max(most, bits) : most;
+        least = counts ? min(least, bits) : least;
+        others |= counts ? bits & 0x7fffff : 0;
+    }
+    // pages `first` .. `last` of a sequence, every stride-th of them
+    template <typename V>
+    __device__ __forceinline__ void look(const V &view, int first, int last, int stride) {
+#pragma unroll 4
+        for (int i = first; i <= last; i += stride) {
+            const uint32_t page = static_cast<uint32_t>(view.table[static_cast<uint32_t>(i)]);
+            take(step_of(view, page), view.has(page));
+        }
+    }
+    // the whole wavefront's
+    __device__ __forceinline__ void join() {
+#pragma unroll
+        for (int d = kWave / 2; d > 0; d /= 2) {
+            most = max(most, __shfl_xor(most, d, kWave));
+            least = min(least, __shfl_xor(least, d, kWave));
+        }
+        most = __builtin_amdgcn_readfirstlane(most);
+        least = __builtin_amdgcn_readfirstlane(least);
+        others = __any(others != 0);
+    }
+    __device__ __forceinline__ int exponent() const { return (most >> 23) - 127; }
+    __device__ __forceinline__ bool far() const { return (most >> 23) - (least >> 23) > kSpread || others != 0; }
 };
 
 template <typename T>
@@ -536,10 +553,8 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     rows.load(g, p.s, p.kv, p.r0, p.rows);
     Softmax<T, D, NT> soft;
     soft.clear();
-    Steps steps;
-    int step_exp = -200;       // E: log2 of the largest step of V met so far
-
     const View<D> view(g, p.s, p.seq, p.kv);
+    int step_exp = 0;          // E
     // pages of the tokens whose K rows (by lane column) and whose V columns (by lane group) a lane loads
     auto pages_of = [&](int t0, uint32_t &pk, uint32_t &pv) {
         pk = view.page_of(t0 + (col / 4) * 16);
@@ -565,11 +580,6 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     auto compute = [&](const Tile<D> &t, int t0) {
         // V's steps relative to the largest; a step that is no number marks the scores instead
         const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
-        steps.take(t.v_scale, odd);
-        if (steps.most > step_exp) {
-            soft.rescale(ldexpf(1.f, step_exp - steps.most));
-            step_exp = steps.most;
-        }
         const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -step_exp));
         const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
         const h2 vf = {f1, f1}, vbias = {b1, b1};
@@ -588,54 +598,70 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
     // numbers of the one after that besides
     constexpr int kStride = kTileKeys * WAVES;
     int t0 = p.begin + wave * kTileKeys;
+    int unit[NT] = {};         // of the outputs, a row's
     if (t0 < p.end) {
+        // the steps' pages come beside the first tile's, the steps beside the tile
+        constexpr int kAhead = 4;
+        const int first = (p.begin >> view.shift) + lane, last = view.page_at((p.end - 1) | (kTileKeys - 1));
+        uint32_t ahead[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            ahead[i] = static_cast<uint32_t>(view.table[static_cast<uint32_t>(min(first + i * kWave, last))]);
         Tile<D> one, two;
         uint32_t pk, pv;
         pages_of(t0, pk, pv);
         uint32_t next_pk = 0, next_pv = 0;
         if (t0 + kStride < p.end) pages_of(t0 + kStride, next_pk, next_pv);
-        fetch(one, t0, pk, pv);
-        while (true) {
-            auto half_step = [&](Tile<D> &now, Tile<D> &next) {
-                const int t1 = t0 + kStride, t2 = t1 + kStride;
-                const bool more = t1 < p.end;
-                if (more) {
-                    const uint32_t a = next_pk, b = next_pv;
-                    if (t2 < p.end) pages_of(t2, next_pk, next_pv);
-                    fetch(next, t1, a, b);
-                }
-                compute(now, t0);
-                t0 = t1;
-                return more && !steps.far();
-            };
-            if (!half_step(one, two)) break;
-            if (!half_step(two, one)) break;
-        }
-    }
-    // steps that lie too far apart: all over again
-    int unit[NT];
+        Steps steps;
+        float step[kAhead];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) unit[n] = step_exp;
-    if (__builtin_expect(steps.far(), 0)) {
-        typename Softmax<T, D, NT>::Reference num;
-        soft.clear(num);
-        for (t0 = p.begin + wave * kTileKeys; t0 < p.end; t0 += kStride) {
-            Tile<D> t;
-            uint32_t pk, pv;
-            pages_of(t0, pk, pv);
-            fetch(t, t0, pk, pv);
-            const bool marked = !(fabsf(t.v_scale) <= 3.402823466e38f) && !t.bad;
-            soft.wide_tile(
-                rows,
-                [&](int j, int q) {
-                    const u32x4 raw = t.k[j][q / 2];
-                    return q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
-                },
-                [&](int d, int hh) { return widen(t.v[d][2 * hh], t.v[d][2 * hh + 1]); },
-                marked ? __uint_as_float(0x7fc00000u) : t.k_scale, t.v_scale, t0,
-                t0 + kTileKeys > p.least || __any(t.bad), t.bad, num);
+        for (int i = 0; i < kAhead; ++i) step[i] = steps.step_of(view, ahead[i]);
+        fetch(one, t0, pk, pv);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) steps.take(step[i], view.has(ahead[i]));
+        steps.look(view, first + kAhead * kWave, last, kWave);
+        steps.join();
+        step_exp = steps.exponent();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) unit[n] = step_exp;
+        if (__builtin_expect(steps.far(), 0)) {
+            typename Softmax<T, D, NT>::Reference num;
+            soft.clear(num);
+            for (; t0 < p.end; t0 += kStride) {
+                Tile<D> t;
+                uint32_t pk, pv;
+                pages_of(t0, pk, pv);
+                fetch(t, t0, pk, pv);
+                const bool marked = !(fabsf(t.v_scale) <= 3.402823466e38f) && !t.bad;
+                soft.wide_tile(
+                    rows,
+                    [&](int j, int q) {
+                        const u32x4 raw = t.k[j][q / 2];
+                        return q % 2 ? widen(raw[2], raw[3]) : widen(raw[0], raw[1]);
+                    },
+                    [&](int d, int hh) { return widen(t.v[d][2 * hh], t.v[d][2 * hh + 1]); },
+                    marked ? __uint_as_float(0x7fc00000u) : t.k_scale, t.v_scale, t0,
+                    t0 + kTileKeys > p.least || __any(t.bad), t.bad, num);
+            }
+            soft.close_range(num, unit);
+        } else {
+            while (true) {
+                auto half_step = [&](Tile<D> &now, Tile<D> &next) {
+                    const int t1 = t0 + kStride, t2 = t1 + kStride;
+                    const bool more = t1 < p.end;
+                    if (more) {
+                        const uint32_t a = next_pk, b = next_pv;
+                        if (t2 < p.end) pages_of(t2, next_pk, next_pv);
+                        fetch(next, t1, a, b);
+                    }
+                    compute(now, t0);
+                    t0 = t1;
+                    return more;
+                };
+                if (!half_step(one, two)) break;
+                if (!half_step(two, one)) break;
+            }
         }
-        soft.close_range(num, unit);
     }
 
     // a wavefront's own mean first (bounded by the largest |v|), then the mean of the means
@@ -734,7 +760,6 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     // what every wavefront knows of a tile whose V is in LDS
     struct Ready {
         float kc;
-        int step_exp;          // E: log2 of the largest step of V met so far, the same in all wavefronts
         bool bad;
     };
     Steps steps;
@@ -750,8 +775,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
     };
     auto widen_v = [&](const Raw &t, int buf) {
         const bool odd = !(fabsf(t.v_scale) <= 3.402823466e38f) || t.bad;
-        steps.take(t.v_scale, odd);
-        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -steps.most));
+        const _Float16 f1 = static_cast<_Float16>(odd ? 0.f : ldexpf(t.v_scale, -steps.exponent()));
         const _Float16 b1 = static_cast<_Float16>(-1152.f) * f1;
         const h2 vf = {f1, f1}, vbias = {b1, b1};
         u32x4 *to = v_lds + buf * kVFrags * kWave;
@@ -761,11 +785,53 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
             for (int hh = 0; hh < 2; ++hh)
                 to[((wave * DW + d) * 2 + hh) * kWave] =
                     __builtin_bit_cast(u32x4, widen_scaled(t.v[d][2 * hh], t.v[d][2 * hh + 1], vf, vbias));
-        return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, steps.most, t.bad};
+        return Ready{odd && !t.bad ? __uint_as_float(0x7fc00000u) : t.k_scale, t.bad};
     };
 
-    int my_exp = -200, unit[NT] = {};
+    int unit[NT] = {};       // of the outputs, a row's
     if (p.begin < p.end) {
+        // each wavefront looks over a quarter of the pages' steps
+        int *const shares = reinterpret_cast<int *>(frags);
+        steps.look(view, (p.begin >> view.shift) + tid, view.page_at((p.end - 1) | (kTileKeys - 1)), kManyWaves * kWave);
+        steps.join();
+        if (lane < 3) shares[wave * 3 + lane] = lane == 0 ? steps.most : lane == 1 ? steps.least : steps.others;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kManyWaves; ++w) {
+            steps.most = max(steps.most, __builtin_amdgcn_readfirstlane(shares[w * 3]));
+            steps.least = min(steps.least, __builtin_amdgcn_readfirstlane(shares[w * 3 + 1]));
+            steps.others |= __builtin_amdgcn_readfirstlane(shares[w * 3 + 2]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) unit[n] = steps.exponent();
+    }
+    if (__builtin_expect(p.begin < p.end && steps.far(), 0)) {
+        // one tile after the other
+        Raw raw;
+        typename Softmax<T, D, NT>::Reference num;
+        soft.clear(num);
+        for (int t0 = p.begin; t0 < p.end; t0 += kTileKeys) {
+            fetch_k(raw, t0, k_page(t0));
+            fetch_v(raw, t0, v_page(t0));
+            __syncthreads();      // everyone has read what the buffers hold
+            widen_k(raw, 0);
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+                    v_lds[((wave * DW + d) * 2 + hh) * kWave] =
+                        __builtin_bit_cast(u32x4, widen(raw.v[d][2 * hh], raw.v[d][2 * hh + 1]));
+            __syncthreads();
+            const bool marked = !(fabsf(raw.v_scale) <= 3.402823466e38f) && !raw.bad;
+            soft.wide_tile(
+                rows, [&](int j, int q) { return __builtin_bit_cast(h8, k_lds[(j * KH + q) * kWave]); },
+                [&](int d, int hh) { return __builtin_bit_cast(h8, v_lds[(d * 2 + hh) * kWave]); },
+                marked ? __uint_as_float(0x7fc00000u) : raw.k_scale, raw.v_scale, t0,
+                t0 + kTileKeys > my_least || __any(raw.bad), raw.bad, num);
+        }
+        soft.close_range(num, unit);
+    } else if (p.begin < p.end) {
         // K is one tile ahead of V: a tile's scores are computed beside the weights of the tile before it, so that
         // the matrix cores and the other units have work at the same time. (Past the last tile the scores are of
         // what the buffer happens to hold, and are not used.)
@@ -796,10 +862,6 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
             __syncthreads();      // V of this tile and K of the next are in LDS, the other buffers have been read by everyone
             // (a wavefront whose rows see nothing of the tile goes along: the branch around it cost more, in copies
             // of the accumulators where its two sides meet)
-            if (ready.step_exp > my_exp) {
-                soft.rescale(ldexpf(1.f, my_exp - ready.step_exp));
-                my_exp = ready.step_exp;
-            }
             float c[NT];
             soft.refer(rows, sc, c, ready.kc, t0, t1 > my_least || __any(ready.bad), ready.bad);
             const u32x4 *v = v_lds + buf * kVFrags * kWave;
@@ -826,33 +888,6 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void attend_many_kernel(Atten
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) sc[j][n] = next[j][n];
-        }
-        // steps that lie too far apart: all over again, one tile after the other
-#pragma unroll
-        for (int n = 0; n < NT; ++n) unit[n] = my_exp;
-        if (__builtin_expect(steps.far(), 0)) {
-            typename Softmax<T, D, NT>::Reference num;
-            soft.clear(num);
-            for (int t0 = p.begin; t0 < p.end; t0 += kTileKeys) {
-                fetch_k(raw, t0, k_page(t0));
-                fetch_v(raw, t0, v_page(t0));
-                __syncthreads();      // everyone has read what the buffers hold
-                widen_k(raw, 0);
-#pragma unroll
-                for (int d = 0; d < DW; ++d)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-                        v_lds[((wave * DW + d) * 2 + hh) * kWave] =
-                            __builtin_bit_cast(u32x4, widen(raw.v[d][2 * hh], raw.v[d][2 * hh + 1]));
-                __syncthreads();
-                const bool marked = !(fabsf(raw.v_scale) <= 3.402823466e38f) && !raw.bad;
-                soft.wide_tile(
-                    rows, [&](int j, int q) { return __builtin_bit_cast(h8, k_lds[(j * KH + q) * kWave]); },
-                    [&](int d, int hh) { return __builtin_bit_cast(h8, v_lds[(d * 2 + hh) * kWave]); },
-                    marked ? __uint_as_float(0x7fc00000u) : raw.k_scale, raw.v_scale, t0,
-                    t0 + kTileKeys > my_least || __any(raw.bad), raw.bad, num);
-            }
-            soft.close_range(num, unit);
         }
     }
 #pragma unroll
