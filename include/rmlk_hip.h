@@ -649,7 +649,8 @@ int32_t rmlk_hip_gemv_kmajor_head_rows(rmlk_stream_t stream, int32_t dtype, int6
 
 /* ---- 8-bit serving: int8 rows, int8 products, a paged int8 cache ------------------------------------
  * Activations (`dtype`: x, q, k, v, residual and the outputs of that kind) are FLOAT, FLOAT16 or
- * BFLOAT16; sums, softmax statistics and norms are formed in 32 bits or more and rounded once. No
+ * BFLOAT16; sums, softmax statistics and norms are formed in 32 bits or more and rounded once (the
+ * attention says what its weights are rounded to before they are multiplied). No
  * counterpart in the reference, whose kernels hold fp32 only.
  *
  * rmlk_hip_quantize_rows: one scale per row (a token's activations, or an output channel's weights),
@@ -731,7 +732,8 @@ typedef struct rmlk_paged_batch {
  * token's position in its sequence (both NULL: k as it is; a token at a position >= positions is
  * skipped and reported, as is a sequence of fewer tokens than rows). A block's scale becomes the
  * smallest power of two s with |x| <= 127 s for everything appended to it, at least 2^-126; an append
- * that starts at slot 0 of a page starts its blocks anew, whatever they held. Rounding to nearest even,
+ * that starts at slot 0 of a page starts its blocks anew, whatever they held; one that goes on with a
+ * block takes the scale it has as a power of two (of its exponent). Rounding to nearest even,
  * decided as in exact arithmetic. A NaN or an infinity among a block's new values makes its scale NaN
  * until the block is started anew, and the attention of every query that sees a token of the block NaN.
  * q (NULL: none), [rows, heads, head_dim], is rotated alike into the dense q_out (may be q where that is

@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kWideWaves *kWave) void int8_wide_kernel(Int8Args<T
 // dealt out between the MFMAs. Rows behind m and n are read from the last row and not stored.
 // 4096 x 8192 x 8192 in tiles of 256 x 256: 250 us, 2200 TOP/s, where the library's product reaches 2430 and the
 // matrix pipes are busy half of the cycles (a higher share lowers the clock). 509 x 8192 x 2048 in 256 tiles of
-// 128 x 128: 13.4 us; a K step takes 0.58 us, the time in which the L2s give a compute unit its 32 KB (14.5
-// TB/s in all), launch and first step 3.3 us, the stores 2 us. Measured and dropped there: 2 x 2
+// 128 x 128: 13.4 - 13.9 us; a K step takes 0.58 us, 32 KB per compute unit from the L2s (14.5 TB/s in all; whether
+// that is the L2s' limit has not been shown), launch and first step 3.3 us, the stores 2 us. Measured and dropped there: 2 x 2
 // wavefronts (17.8 us at the time of 17.3), 64 x 128 tiles, two blocks per compute unit (20.3 us), two stages (23.2).
 // Rows of a and wt that start inside a cache line make every step's 128 bytes cross from the L2 as two lines:
 // 635 x 26100 x 3550 takes 124 us with a pitch of 3552, 95 us with one of 3584.

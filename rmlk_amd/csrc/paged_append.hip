@@ -149,7 +149,7 @@ __device__ __forceinline__ void store_rotated(T *to, int half, const float (&a)[
 // rotate q.
 // Single tokens are a chain of trips to memory (the sequence, its page, values and scales): 64 of them, 8 KV heads
 // of 64 dims, 5.1 us. Prompts are bound by the bytes and by that chain in about equal parts: 2275 tokens of 8
-// sequences in bfloat16, 8 KV heads of 128 dims and 32 heads of q (53.6 MB) take 18.1 us, 13 us without q.
+// sequences in bfloat16, 8 KV heads of 128 dims and 32 heads of q (53.6 MB) take 18.2 us, 13 us without q.
 // Measured and dropped: K and V in blocks of their own (20.8 became 26 us), units of 4 + 4 dims (25 us), q by
 // one or four heads per thread (1.1 us more; 2.2 us more with single tokens). Queries of 16-bit types turned in
 // double took 22.5 us when float took 20.8, plain stores of them 20.8 where streaming ones take 18.1 (with the

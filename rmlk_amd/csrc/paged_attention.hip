@@ -539,8 +539,9 @@ __device__ __forceinline__ bool find_place(const AttendArgs<T> &g, int tile_rows
 
 // Few rows (16 * NT of them): the wavefronts of a block deal the tiles of keys out among themselves, everything
 // in registers. Bound by the cache's bytes: 64 single tokens behind 100 .. 16384 keys (8 KV heads of 128 dims, 415
-// MB) take 91 us with the join, 4.5 TB/s, where a large copy reaches 5.1. A single token behind 640 keys takes
-// 7.5 us, a chain of trips to memory (the sequence, its pages, three tiles per wavefront, the wavefronts' meeting).
+// MB) take 90 us with the join, 4.6 TB/s, where a large copy reaches 5.1. A single token behind 640 keys takes
+// 7.5 us, a chain of trips to memory: the sequence, its pages, the two or three tiles that each of the four wavefronts
+// of its eight blocks (one per KV head) takes one after the other, the wavefronts' meeting.
 template <typename T, int D, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<T> g) {
     constexpr int DT = D / 16, KC = D / 64, R = 16 * NT, kPad = D + 4;
@@ -706,13 +707,14 @@ __global__ __launch_bounds__(WAVES *kWave, 2) void attend_few_kernel(AttendArgs<
 // Many rows: four wavefronts of 16 * NT rows each walk the same tiles of keys. A wavefront fetches and widens a
 // quarter of a tile and leaves it in LDS as the MFMA operands it is (64 lanes x 16 bytes each, read back as
 // they were written: no bank conflicts); two buffers, one barrier per tile. What widening costs, and the
-// trips to the caches, are shared by the block's rows. Bound by the issue of instructions: beside the 64 MFMAs of
-// a tile (D = 128, 16-bit types) a wavefront has some 270 vector instructions (32 exponentials and as many
+// trips to the caches, are shared by the block's rows. Neither pipe is full: a prompt of 8192 tokens has the vector
+// pipes busy 63 % and the matrix pipes 42 % of the cycles, 2048 tokens of 64 dims in floats 45 and 25 %. Beside the 64
+// MFMAs of a tile (D = 128, 16-bit types) a wavefront has some 270 vector instructions (32 exponentials and as many
 // arguments and maxima, the widening, addresses), and only a part of them runs under MFMAs: with two wavefronts per
 // SIMD, sixteen v_mfma_f32_16x16x32_f16 each take 541 cycles alone, 578, 595, 713 and 825 with one to four
 // multiply-adds behind every one of them, 566 with an exponential. So the scores of the next tile are computed beside
-// the weights of this one (a prompt of 8192 tokens, 32 heads of 128 dims: 627 us without, 585 us so, 940
-// TFLOP/s of the causal half), the largest score is looked for before the factors are applied, and an address is
+// the weights of this one (a prompt of 8192 tokens, 32 heads of 128 dims: 627 us without when it took 585 so; now
+// 576, 955 TFLOP/s of the causal half), the largest score is looked for before the factors are applied, and an address is
 // one wide multiply. Measured and dropped: wavefront priorities (592 us), orders of MFMAs and vector instructions
 // given to the compiler (no faster), branches around the last fetch (the registers they hold).
 constexpr int kManyWaves = 4;
